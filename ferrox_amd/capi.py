@@ -6,6 +6,7 @@ benchmark read like the C calls they make.  There is no CPU fallback: if the lib
 import raises.
 """
 import ctypes as C
+import math
 import os
 
 import numpy as np
@@ -21,6 +22,7 @@ UNARY_OPS = {"neg": 0, "sqrt": 1, "exp": 2, "log": 3, "relu": 4, "sigmoid": 5, "
              "sign": 9, "logical_not": 10}
 SCALAR_OPS = {"add_scalar": 0, "sub_scalar": 1, "mul_scalar": 2, "div_scalar": 3, "greater_scalar": 4,
               "greater_equal_scalar": 5, "less_equal_scalar": 6, "less_scalar": 7, "pow_scalar": 8}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 FX_MAX_BUCKETS = 8
 
 
@@ -160,6 +162,16 @@ for _s, _ct in (("f32", C.c_float), ("f64", C.c_double)):
 
     _sig(f"fx_adam_step_multi_bc_{_s}", _vp, _int, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp),
          C.POINTER(_i64), *([_ct] * 5), _vp)
+    _sig(f"fx_embedding_fwd_{_s}", _vp, _vp, _vp, _vp, _i64, _i64, _i64, _ct)
+    _sig(f"fx_embedding_bwd_{_s}", _vp, _vp, _vp, _vp, _i64, _i64, _i64, _ct)
+    _sig(f"fx_rmsnorm_fwd_{_s}", _vp, _vp, _vp, _vp, C.c_double, _vp, _vp, _vp, _i64, _i64)
+    _sig(f"fx_rmsnorm_bwd_{_s}", *([_vp] * 8), _i64, _i64)
+    _sig(f"fx_gemm_bias_act_residual_{_s}", _vp, _int, _int, _i64, _i64, _i64, *([_vp] * 6), _int)
+    _sig(f"fx_linear_act_bwd_{_s}", _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp)
+    _sig(f"fx_gated_recurrence_fwd_{_s}", *([_vp] * 5), _i64, _i64, _i64)
+    _sig(f"fx_gated_recurrence_bwd_{_s}", *([_vp] * 10), _i64, _i64, _i64)
+    _sig(f"fx_grad_norm_multi_{_s}", _vp, _int, C.POINTER(_vp), C.POINTER(_i64), _vp)
+    _sig(f"fx_clip_grad_norm_multi_{_s}", _vp, _int, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_i64), C.c_double, _vp)
 
 _sig("fx_graph_begin", _vp)
 _sig("fx_graph_end", _vp, C.POINTER(_vp))
@@ -186,7 +198,17 @@ def check(rc):
         raise FerroxHipError(rc, lib.fx_last_error().decode("utf-8", "replace"))
 
 
+def _ptr(a):
+    return None if a is None else a.ptr
+
+
+_DTYPE_CODES = {np.dtype(np.float32): (FX_F32, "f32"), np.dtype(np.float64): (FX_F64, "f64")}
+
+
 def dtype_code(dtype):
+    code = _DTYPE_CODES.get(dtype)
+    if code is not None:
+        return code
     dtype = np.dtype(dtype)
     if dtype == np.float32:
         return FX_F32, "f32"
@@ -204,7 +226,7 @@ class DeviceArray:
 
     @property
     def size(self):
-        return int(np.prod(self.shape, dtype=np.int64))
+        return math.prod(self.shape)
 
     @property
     def nbytes(self):
@@ -641,6 +663,151 @@ class Context:
 
     def sgd_step(self, p, g, lr):
         check(self._fn("sgd_step", p.dtype)(self.h, p.ptr, g.ptr, p.size, lr))
+
+    # ---- a language model's training step (`out`: the caller's own output arrays, None: from the pool)
+    def upload_ids(self, ids):
+        """Token ids on the device (int64) for embedding_fwd / embedding_bwd; any shape, read in order."""
+        ids = np.ascontiguousarray(ids, dtype=np.int64)
+        d = _RawI64(self, max(1, ids.size))
+        d.shape = ids.shape
+        if ids.size:
+            check(lib.fx_h2d(self.h, d.ptr, ids.ctypes.data_as(_vp), ids.nbytes))
+        return d
+
+    def _same(self, what, want, dtype, **arrays):
+        """Every array given has this shape and type; the C calls cannot see either."""
+        for name, a in arrays.items():
+            if a is not None and (a.shape != tuple(want) or a.dtype != dtype):
+                raise FerroxHipError(1, f"{what}: {name} is {a.shape} {a.dtype}, not {tuple(want)} {dtype}")
+
+    def embedding_fwd(self, w, ids, scale=1.0, out=None):
+        """out[..., :] = scale * w[ids[...], :]; zeros where an id lies outside the table."""
+        vocab, dim = w.shape
+        shape = tuple(ids.shape) + (dim,)
+        n = math.prod(ids.shape)
+        if out is None:
+            out = self.empty(shape, w.dtype)
+        self._same("embedding_fwd", shape, w.dtype, out=out)
+        check(self._fn("embedding_fwd", w.dtype)(self.h, w.ptr, ids.ptr, out.ptr, n, vocab, dim, float(scale)))
+        return out
+
+    def embedding_bwd(self, g, ids, vocab, scale=1.0, out=None):
+        """The dense gradient [vocab, dim] of the table from g, the gradient of embedding_fwd's output."""
+        dim = g.shape[-1]
+        n = math.prod(ids.shape)
+        self._same("embedding_bwd", tuple(ids.shape) + (dim,), g.dtype, g=g)
+        if out is None:
+            out = self.empty((vocab, dim), g.dtype)
+        self._same("embedding_bwd", (vocab, dim), g.dtype, out=out)
+        check(self._fn("embedding_bwd", g.dtype)(self.h, g.ptr, ids.ptr, out.ptr, n, vocab, dim, float(scale)))
+        return out
+
+    def rmsnorm_fwd(self, x, w, eps, res=None, out=None):
+        """(h, y, rstd): h = x + res (None without res), y = h / rms(h) * w over the last axis, rstd one value per row."""
+        dim = x.shape[-1]
+        rows = math.prod(x.shape[:-1])
+        if out is None:
+            out = (self.empty(x.shape, x.dtype) if res is not None else None, self.empty(x.shape, x.dtype), self.empty((rows,), x.dtype))
+        h, y, rstd = out
+        self._same("rmsnorm_fwd", x.shape, x.dtype, res=res, h=h, y=y)
+        self._same("rmsnorm_fwd", (dim,), x.dtype, w=w)
+        self._same("rmsnorm_fwd", (rows,), x.dtype, rstd=rstd)
+        check(self._fn("rmsnorm_fwd", x.dtype)(self.h, x.ptr, _ptr(res), w.ptr, float(eps), _ptr(h), y.ptr, _ptr(rstd), rows, dim))
+        return h, y, rstd
+
+    def rmsnorm_bwd(self, dy, h, w, rstd, dh=None, want_dw=True, out=None):
+        """(dx, dw) from the gradients of y and (dh) of h; dx is the gradient of x and of res."""
+        dim = dy.shape[-1]
+        rows = math.prod(dy.shape[:-1])
+        if out is None:
+            out = (self.empty(dy.shape, dy.dtype), self.empty((dim,), dy.dtype) if want_dw else None)
+        dx, dw = out
+        self._same("rmsnorm_bwd", dy.shape, dy.dtype, h=h, dh=dh, dx=dx)
+        self._same("rmsnorm_bwd", (dim,), dy.dtype, w=w, dw=dw)
+        self._same("rmsnorm_bwd", (rows,), dy.dtype, rstd=rstd)
+        check(self._fn("rmsnorm_bwd", dy.dtype)(self.h, dy.ptr, _ptr(dh), h.ptr, w.ptr, rstd.ptr, dx.ptr, _ptr(dw), rows, dim))
+        return dx, dw
+
+    def gemm_bias_act_residual(self, a, b, ta=False, tb=False, bias=None, act="none", residual=None, pre=None, out=None):
+        """act(op(a) . op(b) + bias) + residual; pre (optional, [M, N]) receives act's argument."""
+        M, K = (a.shape[1], a.shape[0]) if ta else a.shape
+        N, Kb = b.shape if tb else (b.shape[1], b.shape[0])
+        if K != Kb:
+            raise FerroxHipError(1, f"Matrix multiplication shape mismatch: ({M}, {K}) @ ({Kb}, {N})")
+        if out is None:
+            out = self.empty((M, N), a.dtype)
+        self._same("gemm_bias_act_residual", (M, N), a.dtype, residual=residual, pre=pre, out=out)
+        self._same("gemm_bias_act_residual", (N,), a.dtype, bias=bias)
+        self._same("gemm_bias_act_residual", b.shape, a.dtype, b=b)
+        check(self._fn("gemm_bias_act_residual", a.dtype)(self.h, int(ta), int(tb), M, N, K, a.ptr, b.ptr, _ptr(bias), _ptr(residual), _ptr(pre),
+                                                          out.ptr, ACTIVATIONS[act]))
+        return out
+
+    def linear_act_bwd(self, dy, w, x, pre, act, want_db=True, out=None):
+        """(dx, dw, db, dpre) of y = act(x . w^T + b) + residual from dy and the saved pre-activation; w is [out, in]."""
+        Bn, O = dy.shape
+        I = w.shape[1]
+        if out is None:
+            out = (self.empty((Bn, I), dy.dtype), self.empty((O, I), dy.dtype), self.empty((O,), dy.dtype) if want_db else None,
+                   self.empty((Bn, O), dy.dtype))
+        dx, dw, db, dpre = out
+        self._same("linear_act_bwd", (Bn, O), dy.dtype, pre=pre, dpre=dpre)
+        self._same("linear_act_bwd", (O, I), dy.dtype, w=w, dw=dw)
+        self._same("linear_act_bwd", (Bn, I), dy.dtype, x=x, dx=dx)
+        self._same("linear_act_bwd", (O,), dy.dtype, db=db)
+        check(self._fn("linear_act_bwd", dy.dtype)(self.h, Bn, I, O, dy.ptr, w.ptr, x.ptr, pre.ptr, ACTIVATIONS[act], dpre.ptr, dx.ptr, dw.ptr,
+                                                   _ptr(db)))
+        return dx, dw, db, dpre
+
+    def gated_recurrence_fwd(self, z, x, h0=None, out=None):
+        """h [B, steps, dim] with h_t = f h_{t-1} + (1 - f) x_t, f = sigmoid(z_t), from the state h0 [B, dim] (None: zeros)."""
+        B, T, D = z.shape
+        if out is None:
+            out = self.empty((B, T, D), z.dtype)
+        self._same("gated_recurrence_fwd", (B, T, D), z.dtype, x=x, out=out)
+        self._same("gated_recurrence_fwd", (B, D), z.dtype, h0=h0)
+        check(self._fn("gated_recurrence_fwd", z.dtype)(self.h, z.ptr, x.ptr, _ptr(h0), out.ptr, B, T, D))
+        return out
+
+    def gated_recurrence_bwd(self, dh, z, x, h, h0=None, dh_next=None, want_dh0=None, out=None):
+        """(dz, dx, dh0); dh0 is None unless there is an h0 or it is asked for."""
+        B, T, D = dh.shape
+        if out is None:
+            want = h0 is not None if want_dh0 is None else want_dh0
+            out = (self.empty(dh.shape, dh.dtype), self.empty(dh.shape, dh.dtype), self.empty((B, D), dh.dtype) if want else None)
+        dz, dx, dh0 = out
+        self._same("gated_recurrence_bwd", (B, T, D), dh.dtype, z=z, x=x, h=h, dz=dz, dx=dx)
+        self._same("gated_recurrence_bwd", (B, D), dh.dtype, h0=h0, dh_next=dh_next, dh0=dh0)
+        check(self._fn("gated_recurrence_bwd", dh.dtype)(self.h, dh.ptr, z.ptr, x.ptr, h.ptr, _ptr(h0), _ptr(dh_next), dz.ptr, dx.ptr, _ptr(dh0),
+                                                         B, T, D))
+        return dz, dx, dh0
+
+    def grad_norm(self, gs, norm=None):
+        """sqrt of the sum of squares over all tensors of the list, as a device array of one element."""
+        return self._grad_norm("grad_norm", gs, None, None, norm)
+
+    def clip_grad_norm(self, gs, max_norm, outs=None, norm=None):
+        """Scales the tensors by max_norm / norm where norm > max_norm (in place, or into outs); returns the norm (device)."""
+        return self._grad_norm("clip_grad_norm", gs, gs if outs is None else outs, max_norm, norm)
+
+    def _grad_norm(self, what, gs, outs, max_norm, norm):
+        k = len(gs)
+        dt = gs[0].dtype if k else (norm.dtype if norm is not None else np.dtype(np.float32))
+        if outs is not None and len(outs) != k:
+            raise FerroxHipError(1, f"{what}: {len(outs)} outputs for {k} tensors")
+        for g, o in zip(gs, gs if outs is None else outs):
+            if g.dtype != dt or o.dtype != dt or o.shape != g.shape:
+                raise FerroxHipError(1, f"{what}: {g.shape} {g.dtype} into {o.shape} {o.dtype}, in a call of {dt}")
+        if norm is None:
+            norm = self.empty((1,), dt)
+        self._same(what, (1,), dt, norm=norm)
+        tab = lambda arrs: (C.c_void_p * k)(*[a.ptr for a in arrs])  # noqa: E731
+        ns = (C.c_int64 * k)(*[a.size for a in gs])
+        if outs is None:
+            check(self._fn("grad_norm_multi", dt)(self.h, k, tab(gs), ns, norm.ptr))
+        else:
+            check(self._fn("clip_grad_norm_multi", dt)(self.h, k, tab(gs), tab(outs), ns, float(max_norm), norm.ptr))
+        return norm
 
     def conv2d_last_path(self):
         """The kernel family the last convolution call on this context ran (a fixed string per dispatch branch)."""

@@ -83,6 +83,11 @@ int bind_device(int device);  // runtime.hip
 #endif
 
 inline i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
+// [a, a + an) and [b, b + bn) elements share memory (null pointers and empty ranges share nothing)
+template <typename T> inline bool overlap(const T* a, i64 an, const T* b, i64 bn) {
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    return a && b && an > 0 && bn > 0 && a0 < b0 + (uintptr_t)bn * sizeof(T) && b0 < a0 + (uintptr_t)an * sizeof(T);
+}
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace fx

@@ -7,6 +7,7 @@
 #include "gemm_lds.hpp"
 #include "gemm_thin.hpp"
 #include "gemm_small.hpp"
+#include "gemm_epilogue.hpp"
 
 extern "C" int fx_bias_act_f32(fx_ctx*, float*, const float*, int64_t, int64_t, int64_t, int);
 extern "C" int fx_bias_act_f64(fx_ctx*, double*, const double*, int64_t, int64_t, int64_t, int);
@@ -215,4 +216,37 @@ extern "C" int fx_gemm_bias_act_f64(fx_ctx* c, int ta, int tb, int64_t M, int64_
     FX_REQUIRE(bias != nullptr, "fx_gemm_bias_act: null bias");
     FX_REQUIRE(act == 0 || act == 1, "fx_gemm_bias_act: act must be 0 (none) or 1 (relu)");
     return gemm<double>(c, ta, tb, M, N, K, A, B, C, bias, act);
+}
+// C = act(op(A).op(B) + bias[n]) + residual, with act(...)'s argument written to pre: a Linear layer on a residual stream.
+template <typename T>
+int gemm_bias_act_residual(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B, const T* bias, const T* residual, T* pre, T* C,
+                           int act) {
+    FX_CHECK_CTX(c);
+    FX_REQUIRE(act >= fxact::NONE && act <= fxact::SILU, "fx_gemm_bias_act_residual: act must be 0 (none), 1 (relu), 2 (gelu) or 3 (silu)");
+    FX_REQUIRE(M >= 0 && N >= 0 && K >= 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), "fx_gemm_bias_act_residual: bad dimensions");
+    if (M == 0 || N == 0) return FX_OK;
+    FX_REQUIRE(C != nullptr && (K == 0 || (A && B)), "fx_gemm_bias_act_residual: null pointer");
+    const i64 n = M * N;
+    FX_REQUIRE(!fx::overlap(C, n, A, M * K) && !fx::overlap(C, n, B, K * N) && !fx::overlap(C, n, bias, N) && !fx::overlap(C, n, residual, n) &&
+                   !fx::overlap<T>(C, n, pre, n) && !fx::overlap<T>(pre, n, A, M * K) && !fx::overlap<T>(pre, n, B, K * N) &&
+                   !fx::overlap<T>(pre, n, bias, N) && !fx::overlap<T>(pre, n, residual, n),
+               "fx_gemm_bias_act_residual: an output overlaps another tensor of the call");
+    if (K == 0) {  // the empty product
+        std::lock_guard<std::mutex> lk(c->launch_mutex);
+        if (int rc = launch_zero<T>(c, C, n)) return rc;
+    } else if (int rc = gemm<T>(c, ta, tb, M, N, K, A, B, C)) {
+        return rc;
+    }
+    const gep::Epilogue<T> ep{bias, residual, pre, act};
+    if (!ep.any()) return FX_OK;
+    std::lock_guard<std::mutex> lk(c->launch_mutex);
+    return gep::launch_pass<T>(c, C, n, N, ep);
+}
+extern "C" int fx_gemm_bias_act_residual_f32(fx_ctx* c, int ta, int tb, int64_t M, int64_t N, int64_t K, const float* A, const float* B,
+                                             const float* bias, const float* residual, float* pre, float* C, int act) {
+    return gemm_bias_act_residual<float>(c, ta, tb, M, N, K, A, B, bias, residual, pre, C, act);
+}
+extern "C" int fx_gemm_bias_act_residual_f64(fx_ctx* c, int ta, int tb, int64_t M, int64_t N, int64_t K, const double* A, const double* B,
+                                             const double* bias, const double* residual, double* pre, double* C, int act) {
+    return gemm_bias_act_residual<double>(c, ta, tb, M, N, K, A, B, bias, residual, pre, C, act);
 }

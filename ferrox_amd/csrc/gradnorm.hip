@@ -1,0 +1,224 @@
+// The global norm of a list of gradient tensors and their clipping by it, the step between the backward pass and the optimizer
+// (fx_adam_step_multi / fx_sgd_step_multi take the same tables):
+//   norm = sqrt(sum over all tensors and elements of g^2);   out_k = g_k * (norm > max_norm ? max_norm / norm : 1)
+// Two passes over the gradients, bound by memory: the first leaves one partial sum of squares per block, the second adds the
+// partials (every block for itself, in one fixed order, so that all blocks and all runs have the same factor) and scales.  Nothing
+// returns to the host in between, so the pair can be recorded into a graph.
+// Squares are added in f64 whatever the tensors' type: f32 gradients neither overflow nor lose small terms, and the extra work is
+// hidden behind the loads.  Everything is summed in a fixed order, no atomics.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "vecio.hpp"
+
+namespace {
+using namespace vio;
+
+constexpr int NT = 256, CHUNK = 4096, TABLE = 96;  // elements of a chunk; tensors of one launch (the table travels in the arguments)
+constexpr int MAX_PARTIALS = 2048;
+
+template <typename T> struct Tensors {
+    const T* g[TABLE];
+    T* out[TABLE];
+    i64 n[TABLE];
+    unsigned first[TABLE + 1];  // tensor t owns chunks first[t] .. first[t + 1]
+    int count;
+};
+
+// the tensor of a chunk: wave-uniform binary search
+template <typename T> __device__ __forceinline__ int tensor_of(const Tensors<T>& tt, unsigned chunk) {
+    int lo = 0, hi = tt.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tt.first[mid] <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void sum_squares_kernel(const Tensors<T> tt, double* __restrict__ part) {
+    constexpr int V = 16 / (int)sizeof(T), PER = CHUNK / NT / V;
+    __shared__ double sm[NT / 64 + 1];
+    double s = 0.;
+    const unsigned chunks = tt.first[tt.count];
+    for (unsigned q = blockIdx.x; q < chunks; q += gridDim.x) {
+        const int t = tensor_of(tt, q);
+        const i64 at = (i64)(q - tt.first[t]) * CHUNK;
+        const T* g = tt.g[t] + at;
+        const i64 left = tt.n[t] - at;
+        if (left >= CHUNK && ((uintptr_t)g & 15) == 0) {
+            T v[PER][V];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) load<V>(g + (k * NT + threadIdx.x) * V, v[k]);
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+#pragma unroll
+                for (int u = 0; u < V; ++u) s = fma((double)v[k][u], (double)v[k][u], s);
+        } else {
+            for (int j = threadIdx.x; j < CHUNK && j < left; j += NT) s = fma((double)g[j], (double)g[j], s);
+        }
+    }
+    s = block_sum<NT>(s, sm);
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// sqrt of the sum of all partials, the same bits in every block
+__device__ __forceinline__ double norm_of(const double* __restrict__ part, int parts, double* sm) {
+    double s = 0.;
+    for (int j = threadIdx.x; j < parts; j += NT) s = s + part[j];
+    return sqrt(block_sum<NT>(s, sm));
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void norm_kernel(const double* __restrict__ part, int parts, T* __restrict__ norm) {
+    __shared__ double sm[NT / 64 + 1];
+    const double v = norm_of(part, parts, sm);
+    if (threadIdx.x == 0) norm[0] = (T)v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void scale_kernel(const Tensors<T> tt, const double* __restrict__ part, int parts, double max_norm, T* norm) {
+    constexpr int V = 16 / (int)sizeof(T), PER = CHUNK / NT / V;
+    __shared__ double sm[NT / 64 + 1];
+    const double total = norm_of(part, parts, sm);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (T)total;
+    // the factor rounded once to the tensors' type; a norm that is infinite or NaN scales nothing
+    const T coef = total > max_norm && total <= 1.7976931348623157e308 ? (T)(max_norm / total) : T(1);
+    const unsigned chunks = tt.first[tt.count];
+    for (unsigned q0 = blockIdx.x; q0 < chunks; q0 += gridDim.x) {
+        const unsigned q = chunks - 1 - q0;  // from the end: what the first pass read last may still be in the Infinity Cache
+        const int t = tensor_of(tt, q);
+        const i64 at = (i64)(q - tt.first[t]) * CHUNK;
+        const T* g = tt.g[t] + at;
+        T* o = tt.out[t] + at;
+        if (coef == T(1) && g == o) continue;  // in place and nothing to scale
+        const i64 left = tt.n[t] - at;
+        if (left >= CHUNK && (((uintptr_t)g | (uintptr_t)o) & 15) == 0) {
+            T v[PER][V];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) load<V>(g + (k * NT + threadIdx.x) * V, v[k]);
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+#pragma unroll
+                for (int u = 0; u < V; ++u) v[k][u] = v[k][u] * coef;
+                store<V>(o + (k * NT + threadIdx.x) * V, v[k]);
+            }
+        } else {
+            for (int j = threadIdx.x; j < CHUNK && j < left; j += NT) o[j] = g[j] * coef;
+        }
+    }
+}
+
+// Fills the table of the tensors from `base` on (empty ones left out); returns the next tensor that did not fit.
+template <typename T>
+int fill_table(Tensors<T>& tt, int base, int count, const T* const* g, T* const* out, const int64_t* n) {
+    tt.count = 0;
+    i64 chunks = 0;
+    int k = base;
+    for (; k < count && tt.count < TABLE; ++k) {
+        if (n[k] == 0) continue;
+        const i64 more = fx::ceil_div(n[k], (i64)CHUNK);
+        if (chunks + more > 0x7fffffff) break;
+        const int t = tt.count++;
+        tt.g[t] = g[k];
+        tt.out[t] = out ? out[k] : nullptr;
+        tt.n[t] = n[k];
+        tt.first[t] = (unsigned)chunks;
+        chunks += more;
+    }
+    tt.first[tt.count] = (unsigned)chunks;
+    return k;
+}
+
+// No output may share memory with another tensor of the call (its own gradient, exactly, excepted).
+template <typename T>
+int check_overlaps(int count, const T* const* g, T* const* out, const int64_t* n, const T* norm) {
+    struct Span { uintptr_t lo, hi; int k; bool out; };
+    std::vector<Span> spans;
+    spans.reserve(2 * (size_t)count + 1);
+    for (int k = 0; k < count; ++k) {
+        if (n[k] == 0) continue;
+        const uintptr_t bytes = (uintptr_t)n[k] * sizeof(T);
+        spans.push_back({(uintptr_t)out[k], (uintptr_t)out[k] + bytes, k, true});
+        if (g[k] != out[k]) spans.push_back({(uintptr_t)g[k], (uintptr_t)g[k] + bytes, k, false});
+    }
+    spans.push_back({(uintptr_t)norm, (uintptr_t)norm + sizeof(T), count, true});
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    // walking up: the furthest end of the outputs so far, and of everything so far
+    uintptr_t out_end = 0, any_end = 0;
+    for (const Span& s : spans) {
+        FX_REQUIRE(!(s.lo < out_end || (s.out && s.lo < any_end)), "fx_clip_grad_norm_multi: an output overlaps another tensor of the call (tensor %d)", s.k);
+        any_end = std::max(any_end, s.hi);
+        if (s.out) out_end = std::max(out_end, s.hi);
+    }
+    return FX_OK;
+}
+
+// out == null: the norm alone
+template <typename T>
+int grad_norm(fx_ctx* c, int count, const T* const* g, T* const* out, const int64_t* n, double max_norm, T* norm, const char* what) {
+    FX_CHECK_CTX(c);
+    FX_REQUIRE(count >= 0, "%s: negative tensor count", what);
+    FX_REQUIRE(norm != nullptr, "%s: null norm pointer", what);
+    FX_REQUIRE(count == 0 || (g && n), "%s: null table", what);
+    for (int k = 0; k < count; ++k) {
+        FX_REQUIRE(n[k] >= 0, "%s: negative element count", what);
+        FX_REQUIRE(n[k] <= (i64)0x7fffffff * CHUNK, "%s: too many elements in tensor %d", what, k);
+        FX_REQUIRE(n[k] == 0 || (g[k] && (!out || out[k])), "%s: null pointer in tensor %d", what, k);
+    }
+    if (out) {
+        if (int rc = check_overlaps<T>(count, g, out, n, norm)) return rc;
+    }
+    std::lock_guard<std::mutex> lk(c->launch_mutex);
+    Tensors<T> tt;
+    // launches of at most TABLE tensors each; together they leave at most about MAX_PARTIALS partial sums
+    int launches = 0;
+    for (int k = 0; k < count;) {
+        k = fill_table<T>(tt, k, count, g, out, n);
+        if (tt.count) ++launches;
+    }
+    const i64 per_launch = std::max<i64>(1, std::min<i64>(8 * (i64)c->num_cus, MAX_PARTIALS / std::max(1, launches)));
+    double* part = (double*)c->get_scratch(std::max<i64>(1, per_launch * launches) * (i64)sizeof(double));
+    if (!part) return FX_ERR_OOM;
+    i64 parts = 0;
+    for (int k = 0; k < count;) {
+        k = fill_table<T>(tt, k, count, g, out, n);
+        if (!tt.count) continue;
+        const i64 blocks = std::min<i64>(per_launch, tt.first[tt.count]);
+        FX_LAUNCH(dim3((unsigned)blocks), dim3(NT), 0, c->stream, (tt, part + parts), sum_squares_kernel<T>);
+        FX_LAUNCH_CHECK();
+        parts += blocks;
+    }
+    FX_REQUIRE(parts <= 0x7fffffff, "%s: too many tensors", what);
+    if (!out || parts == 0) {
+        FX_LAUNCH(dim3(1), dim3(NT), 0, c->stream, (part, (int)parts, norm), norm_kernel<T>);
+        FX_LAUNCH_CHECK();
+        return FX_OK;
+    }
+    T* norm_out = norm;
+    for (int k = 0; k < count;) {
+        k = fill_table<T>(tt, k, count, g, out, n);
+        if (!tt.count) continue;
+        const i64 blocks = std::min<i64>(8 * (i64)c->num_cus, tt.first[tt.count]);
+        FX_LAUNCH(dim3((unsigned)blocks), dim3(NT), 0, c->stream, (tt, part, (int)parts, max_norm, norm_out), scale_kernel<T>);
+        FX_LAUNCH_CHECK();
+        norm_out = nullptr;
+    }
+    return FX_OK;
+}
+}  // namespace
+
+#define FX_DEFINE_GRADNORM(T, S)                                                                                                       \
+    extern "C" int fx_grad_norm_multi_##S(fx_ctx* c, int count, const T* const* g, const int64_t* n, T* norm) {                         \
+        return grad_norm<T>(c, count, g, nullptr, n, 0., norm, "fx_grad_norm_multi");                                                  \
+    }                                                                                                                                  \
+    extern "C" int fx_clip_grad_norm_multi_##S(fx_ctx* c, int count, const T* const* g, T* const* out, const int64_t* n,                \
+                                               double max_norm, T* norm) {                                                            \
+        FX_REQUIRE(count <= 0 || out, "fx_clip_grad_norm_multi: null table");                                                          \
+        FX_REQUIRE(max_norm >= 0, "fx_clip_grad_norm_multi: max_norm must not be negative");                                          \
+        return grad_norm<T>(c, count, g, out, n, max_norm, norm, "fx_clip_grad_norm_multi");                                           \
+    }
+FX_DEFINE_GRADNORM(float, f32)
+FX_DEFINE_GRADNORM(double, f64)

@@ -1,0 +1,341 @@
+// Root-mean-square norm over the rows of [rows, D] with the residual's addition in front of it, and its backward pass.
+//   forward:   h = x + res;  rstd = (sum_j h_j^2 / D + eps)^(-1/2);  y_j = (h_j rstd) w_j
+//   backward:  dx_j = dh_j + rstd (w_j dy_j) - h_j rstd^3 (sum_k w_k dy_k h_k) / D;  dw_j = sum over rows of dy_j (h_j rstd)
+// Both are bound by memory: 2 reads and 2 writes of [rows, D] forward, 3 reads and 1 write backward.  A row stays in registers
+// between its one read and its one write: up to 16 elements per thread, one wave per row up to 1024 elements, a block of 256 up to
+// 4096 and of 1024 up to 16384; longer rows are read twice.  Rows that are not whole aligned 16-byte vectors are read element by
+// element.  Sums are held in the tensors' own type (f32 or f64): a thread adds at most 16 terms before the tree of its block.
+// The weight gradient is added up in registers over the rows that a block takes (thread t owns the same columns in every row), one
+// partial row per block, and the partial rows are added by a second launch in a fixed order: no atomics.
+#include <mutex>
+
+#include "vecio.hpp"
+
+namespace {
+using namespace vio;
+
+template <typename T> __device__ __forceinline__ T inv_sqrt(T v);
+template <> __device__ __forceinline__ float inv_sqrt<float>(float v) { return 1.f / sqrtf(v); }
+template <> __device__ __forceinline__ double inv_sqrt<double>(double v) { return 1. / sqrt(v); }
+
+constexpr int block_of(int nt) { return nt < 256 ? 256 : nt; }
+
+// NT threads per row, E elements per thread, V per load.
+template <typename T, int V, int NT, int E, bool RES>
+__global__ __launch_bounds__(block_of(NT)) void rmsnorm_fwd_kernel(const T* x, const T* res, const T* __restrict__ w, T eps, T* h, T* y,
+                                                                   T* __restrict__ rstd, i64 rows, int D) {
+    constexpr int BT = block_of(NT), NV = E / V;
+    __shared__ T sm[BT / 64 + 1];
+    const int t = threadIdx.x % NT;
+    const i64 row = (i64)blockIdx.x * (BT / NT) + threadIdx.x / NT;
+    if (row >= rows) return;  // whole waves only: the variants with a barrier have one row per block
+    const i64 base = row * D;
+    T v[NV][V];
+    T s = T(0);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int j = (k * NT + t) * V;
+        if (j < D) {
+            load<V>(x + base + j, v[k]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < V; ++u) v[k][u] = T(0);
+        }
+    }
+    if constexpr (RES) {
+        T r[NV][V];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int j = (k * NT + t) * V;
+            if (j < D) load<V>(res + base + j, r[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int j = (k * NT + t) * V;
+            if (j < D) {
+#pragma unroll
+                for (int u = 0; u < V; ++u) v[k][u] = v[k][u] + r[k][u];
+                store<V>(h + base + j, v[k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int u = 0; u < V; ++u) s = s + v[k][u] * v[k][u];
+    s = block_sum<NT>(s, sm);
+    const T r = inv_sqrt<T>(s / T(D) + eps);
+    if (t == 0 && rstd) rstd[row] = r;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int j = (k * NT + t) * V;
+        if (j < D) {
+            T g[V];
+            load<V>(w + j, g);
+#pragma unroll
+            for (int u = 0; u < V; ++u) g[u] = (v[k][u] * r) * g[u];
+            store<V>(y + base + j, g);
+        }
+    }
+}
+
+// Rows longer than a block's registers: the second pass reads the row again (the sum with the residual from h, where this thread put it).
+template <typename T, bool RES>
+__global__ __launch_bounds__(1024) void rmsnorm_fwd_long_kernel(const T* x, const T* res, const T* __restrict__ w, T eps, T* h, T* y,
+                                                                T* __restrict__ rstd, i64 D) {
+    __shared__ T sm[17];
+    const i64 base = (i64)blockIdx.x * D;
+    T s = T(0);
+    for (i64 j = threadIdx.x; j < D; j += 1024) {
+        T v = x[base + j];
+        if constexpr (RES) {
+            v = v + res[base + j];
+            h[base + j] = v;
+        }
+        s = s + v * v;
+    }
+    s = block_sum<1024>(s, sm);
+    const T r = inv_sqrt<T>(s / T(D) + eps);
+    if (threadIdx.x == 0 && rstd) rstd[blockIdx.x] = r;
+    const T* src = RES ? h : x;
+    for (i64 j = threadIdx.x; j < D; j += 1024) y[base + j] = (src[base + j] * r) * w[j];
+}
+
+template <typename T, int V, int NT, int E>
+int launch_fwd(fx_ctx* c, const T* x, const T* res, const T* w, T eps, T* h, T* y, T* rstd, i64 rows, i64 D) {
+    constexpr int BT = block_of(NT);
+    const i64 blocks = fx::ceil_div(rows, (i64)(BT / NT));
+    FX_REQUIRE(blocks <= 0x7fffffff, "fx_rmsnorm_fwd: too many rows");
+    const dim3 grid((unsigned)blocks), blk(BT);
+    if (res) FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, eps, h, y, rstd, rows, (int)D), rmsnorm_fwd_kernel<T, V, NT, E, true>);
+    else FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, eps, h, y, rstd, rows, (int)D), rmsnorm_fwd_kernel<T, V, NT, E, false>);
+    FX_LAUNCH_CHECK();
+    return FX_OK;
+}
+template <typename T, int V>
+int dispatch_fwd(fx_ctx* c, const T* x, const T* res, const T* w, T eps, T* h, T* y, T* rstd, i64 rows, i64 D) {
+    if (D <= 64 * 4) return launch_fwd<T, V, 64, 4>(c, x, res, w, eps, h, y, rstd, rows, D);
+    if (D <= 64 * 8) return launch_fwd<T, V, 64, 8>(c, x, res, w, eps, h, y, rstd, rows, D);
+    if (D <= 64 * 16) return launch_fwd<T, V, 64, 16>(c, x, res, w, eps, h, y, rstd, rows, D);
+    if (D <= 256 * 8) return launch_fwd<T, V, 256, 8>(c, x, res, w, eps, h, y, rstd, rows, D);
+    if (D <= 256 * 16) return launch_fwd<T, V, 256, 16>(c, x, res, w, eps, h, y, rstd, rows, D);
+    return launch_fwd<T, V, 1024, 16>(c, x, res, w, eps, h, y, rstd, rows, D);
+}
+
+template <typename T>
+int rmsnorm_fwd(fx_ctx* c, const T* x, const T* res, const T* w, double eps, T* h, T* y, T* rstd, i64 rows, i64 D) {
+    FX_CHECK_CTX(c);
+    FX_REQUIRE(rows >= 0 && D >= 1, "fx_rmsnorm_fwd: bad shape [%lld, %lld]", (long long)rows, (long long)D);
+    FX_REQUIRE(eps >= 0, "fx_rmsnorm_fwd: eps must not be negative");
+    if (rows == 0) return FX_OK;
+    FX_REQUIRE(x && w && y, "fx_rmsnorm_fwd: null pointer");
+    FX_REQUIRE((res != nullptr) == (h != nullptr), "fx_rmsnorm_fwd: h is written exactly when a residual is given");
+    FX_REQUIRE(D < (1ll << 31) && rows < (1ll << 31), "fx_rmsnorm_fwd: dimension exceeds 2^31");
+    const i64 n = rows * D;
+    // h and y may be x or res themselves (an element is read by the thread that writes it), nothing may overlap otherwise
+    const T* ins[] = {x, res, w};
+    T* outs[] = {h, y, rstd};
+    for (int o = 0; o < 3; ++o) {
+        const i64 on = o < 2 ? n : rows;
+        for (int i = 0; i < 3; ++i)
+            FX_REQUIRE((o < 2 && i < 2 && outs[o] == ins[i]) || !fx::overlap<T>(outs[o], on, ins[i], i < 2 ? n : D),
+                       "fx_rmsnorm_fwd: an output overlaps an input that it is not");
+        for (int p = 0; p < o; ++p) FX_REQUIRE(!fx::overlap<T>(outs[o], on, outs[p], n), "fx_rmsnorm_fwd: two outputs overlap");
+    }
+    constexpr int V = 16 / (int)sizeof(T);
+    const T e = (T)eps;
+    if (D > 1024 * 16) {
+        const dim3 grid((unsigned)rows), blk(1024);
+        if (res) FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, e, h, y, rstd, D), rmsnorm_fwd_long_kernel<T, true>);
+        else FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, e, h, y, rstd, D), rmsnorm_fwd_long_kernel<T, false>);
+        FX_LAUNCH_CHECK();
+        return FX_OK;
+    }
+    const bool vec = D % V == 0 && fx::aligned16(x) && fx::aligned16(w) && fx::aligned16(y) && (!res || (fx::aligned16(res) && fx::aligned16(h)));
+    return vec ? dispatch_fwd<T, V>(c, x, res, w, e, h, y, rstd, rows, D) : dispatch_fwd<T, 1>(c, x, res, w, e, h, y, rstd, rows, D);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------------
+// Row group g of block b takes rows b * groups + g, + gridDim * groups, ...; part (when the weight gradient is wanted) gets the
+// block's row of partial sums.
+template <typename T, int V, int NT, int E>
+__global__ __launch_bounds__(block_of(NT)) void rmsnorm_bwd_kernel(const T* dy, const T* dh, const T* h, const T* __restrict__ w,
+                                                                   const T* __restrict__ rstd, T* dx, T* __restrict__ part, i64 rows, int D) {
+    constexpr int BT = block_of(NT), NV = E / V, GR = BT / NT;
+    __shared__ T sm[GR > 1 ? GR * NT * E : BT / 64 + 1];
+    const int t = threadIdx.x % NT, group = threadIdx.x / NT;
+    T wv[NV][V], dw[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int j = (k * NT + t) * V;
+#pragma unroll
+        for (int u = 0; u < V; ++u) dw[k][u] = wv[k][u] = T(0);
+        if (j < D) load<V>(w + j, wv[k]);
+    }
+    for (i64 row = (i64)blockIdx.x * GR + group; row < rows; row += (i64)gridDim.x * GR) {
+        const i64 base = row * D;
+        const T r = rstd[row];
+        T g[NV][V], hv[NV][V];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int j = (k * NT + t) * V;
+            if (j < D) {
+                load<V>(dy + base + j, g[k]);
+                load<V>(h + base + j, hv[k]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < V; ++u) g[k][u] = hv[k][u] = T(0);
+            }
+        }
+        T s = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                dw[k][u] = dw[k][u] + g[k][u] * (hv[k][u] * r);
+                g[k][u] = g[k][u] * wv[k][u];
+                s = s + g[k][u] * hv[k][u];
+            }
+        if (GR == 1) __syncthreads();  // the sums of the row before have been read
+        s = block_sum<NT>(s, sm);
+        const T q = (s / T(D)) * (r * r);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int j = (k * NT + t) * V;
+            if (j < D) {
+                T d[V];
+                if (dh) load<V>(dh + base + j, d);
+#pragma unroll
+                for (int u = 0; u < V; ++u) {
+                    const T a = r * (g[k][u] - hv[k][u] * q);
+                    d[u] = dh ? a + d[u] : a;
+                }
+                store<V>(dx + base + j, d);
+            }
+        }
+    }
+    if (!part) return;
+    if constexpr (GR > 1) {  // the groups' sums in group order
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int u = 0; u < V; ++u) sm[group * (NT * E) + (k * NT + t) * V + u] = dw[k][u];
+        __syncthreads();
+        for (int j = threadIdx.x; j < D; j += BT) {
+            T s = sm[j];
+#pragma unroll
+            for (int q = 1; q < GR; ++q) s = s + sm[q * (NT * E) + j];
+            part[(i64)blockIdx.x * D + j] = s;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int j = (k * NT + t) * V;
+            if (j < D) store<V>(part + (i64)blockIdx.x * D + j, dw[k]);
+        }
+    }
+}
+
+// Long rows: dx row by row (the row read twice), the weight gradient by columns below.
+template <typename T>
+__global__ __launch_bounds__(1024) void rmsnorm_bwd_long_kernel(const T* dy, const T* dh, const T* h, const T* __restrict__ w,
+                                                                const T* __restrict__ rstd, T* dx, i64 D) {
+    __shared__ T sm[17];
+    const i64 base = (i64)blockIdx.x * D;
+    const T r = rstd[blockIdx.x];
+    T s = T(0);
+    for (i64 j = threadIdx.x; j < D; j += 1024) s = s + (dy[base + j] * w[j]) * h[base + j];
+    s = block_sum<1024>(s, sm);
+    const T q = (s / T(D)) * (r * r);
+    for (i64 j = threadIdx.x; j < D; j += 1024) {
+        const T a = r * (dy[base + j] * w[j] - h[base + j] * q);
+        dx[base + j] = dh ? a + dh[base + j] : a;
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void rmsnorm_dw_long_kernel(const T* __restrict__ dy, const T* __restrict__ h, const T* __restrict__ rstd,
+                                                              T* __restrict__ part, i64 rows, i64 D) {
+    const i64 j = (i64)blockIdx.x * 256 + threadIdx.x;
+    if (j >= D) return;
+    T s = T(0);
+    for (i64 r = blockIdx.y; r < rows; r += gridDim.y) s = s + dy[r * D + j] * (h[r * D + j] * rstd[r]);
+    part[(i64)blockIdx.y * D + j] = s;
+}
+
+template <typename T, int V, int NT, int E>
+int launch_bwd(fx_ctx* c, const T* dy, const T* dh, const T* h, const T* w, const T* rstd, T* dx, T* dw, i64 rows, i64 D) {
+    constexpr int BT = block_of(NT), GR = BT / NT;
+    // enough blocks to fill the chip and no more: every block leaves a partial row of the weight gradient
+    const i64 per_cu = BT >= 1024 ? 2 : 4;
+    const i64 blocks = std::min<i64>(fx::ceil_div(rows, (i64)GR), per_cu * c->num_cus);
+    T* part = nullptr;
+    if (dw) {
+        part = blocks == 1 ? dw : (T*)c->get_scratch(blocks * D * (i64)sizeof(T));
+        if (!part) return FX_ERR_OOM;
+    }
+    FX_LAUNCH(dim3((unsigned)blocks), dim3(BT), 0, c->stream, (dy, dh, h, w, rstd, dx, part, rows, (int)D), rmsnorm_bwd_kernel<T, V, NT, E>);
+    FX_LAUNCH_CHECK();
+    return dw && blocks > 1 ? column_sum<T>(c, part, dw, (int)blocks, D) : FX_OK;
+}
+template <typename T, int V>
+int dispatch_bwd(fx_ctx* c, const T* dy, const T* dh, const T* h, const T* w, const T* rstd, T* dx, T* dw, i64 rows, i64 D) {
+    if (D <= 64 * 4) return launch_bwd<T, V, 64, 4>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+    if (D <= 64 * 8) return launch_bwd<T, V, 64, 8>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+    if (D <= 64 * 16) return launch_bwd<T, V, 64, 16>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+    if (D <= 256 * 8) return launch_bwd<T, V, 256, 8>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+    if (D <= 256 * 16) return launch_bwd<T, V, 256, 16>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+    return launch_bwd<T, V, 1024, 16>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+}
+
+template <typename T>
+int rmsnorm_bwd(fx_ctx* c, const T* dy, const T* dh, const T* h, const T* w, const T* rstd, T* dx, T* dw, i64 rows, i64 D) {
+    FX_CHECK_CTX(c);
+    FX_REQUIRE(rows >= 0 && D >= 1, "fx_rmsnorm_bwd: bad shape [%lld, %lld]", (long long)rows, (long long)D);
+    FX_REQUIRE(D < (1ll << 31) && rows < (1ll << 31), "fx_rmsnorm_bwd: dimension exceeds 2^31");
+    const i64 n = rows * D;
+    if (rows == 0) {  // the sum over no rows
+        if (!dw) return FX_OK;
+        if constexpr (sizeof(T) == 4) return fx_fill_f32(c, dw, 0.f, D);
+        else return fx_fill_f64(c, dw, 0., D);
+    }
+    FX_REQUIRE(dy && h && w && rstd && dx, "fx_rmsnorm_bwd: null pointer");
+    const T* ins[] = {dy, dh, h, w, rstd};
+    const i64 insz[] = {n, n, n, D, rows};
+    for (int i = 0; i < 5; ++i)
+        FX_REQUIRE(((i < 2 && dx == ins[i]) || !fx::overlap<T>(dx, n, ins[i], insz[i])) && !fx::overlap<T>(dw, D, ins[i], insz[i]),
+                   "fx_rmsnorm_bwd: an output overlaps an input that it is not");
+    FX_REQUIRE(!fx::overlap(dw, D, dx, n), "fx_rmsnorm_bwd: dx and dw overlap");
+    constexpr int V = 16 / (int)sizeof(T);
+    std::lock_guard<std::mutex> lk(c->launch_mutex);
+    if (D > 1024 * 16) {
+        if (dw) {  // first, since dx may be written over dy
+            const i64 slices = std::min<i64>(rows, std::max<i64>(1, 8 * (i64)c->num_cus / fx::ceil_div(D, (i64)256)));
+            T* part = slices == 1 ? dw : (T*)c->get_scratch(slices * D * (i64)sizeof(T));
+            if (!part) return FX_ERR_OOM;
+            FX_LAUNCH(dim3((unsigned)fx::ceil_div(D, (i64)256), (unsigned)slices), dim3(256), 0, c->stream, (dy, h, rstd, part, rows, D), rmsnorm_dw_long_kernel<T>);
+            FX_LAUNCH_CHECK();
+            if (slices > 1) {
+                if (int rc = column_sum<T>(c, part, dw, (int)slices, D)) return rc;
+            }
+        }
+        FX_LAUNCH(dim3((unsigned)rows), dim3(1024), 0, c->stream, (dy, dh, h, w, rstd, dx, D), rmsnorm_bwd_long_kernel<T>);
+        FX_LAUNCH_CHECK();
+        return FX_OK;
+    }
+    const bool vec = D % V == 0 && fx::aligned16(dy) && fx::aligned16(h) && fx::aligned16(w) && fx::aligned16(dx) && (!dh || fx::aligned16(dh)) &&
+                     (!dw || fx::aligned16(dw));
+    return vec ? dispatch_bwd<T, V>(c, dy, dh, h, w, rstd, dx, dw, rows, D) : dispatch_bwd<T, 1>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+}
+}  // namespace
+
+#define FX_DEFINE_RMSNORM(T, S)                                                                                                        \
+    extern "C" int fx_rmsnorm_fwd_##S(fx_ctx* c, const T* x, const T* res, const T* w, double eps, T* h, T* y, T* rstd, int64_t rows,   \
+                                      int64_t D) {                                                                                     \
+        return rmsnorm_fwd<T>(c, x, res, w, eps, h, y, rstd, rows, D);                                                                 \
+    }                                                                                                                                  \
+    extern "C" int fx_rmsnorm_bwd_##S(fx_ctx* c, const T* dy, const T* dh, const T* h, const T* w, const T* rstd, T* dx, T* dw,         \
+                                      int64_t rows, int64_t D) {                                                                       \
+        return rmsnorm_bwd<T>(c, dy, dh, h, w, rstd, dx, dw, rows, D);                                                                 \
+    }
+FX_DEFINE_RMSNORM(float, f32)
+FX_DEFINE_RMSNORM(double, f64)

@@ -390,7 +390,56 @@ enum fx_scalar_op { FX_ADD_SCALAR = 0, FX_SUB_SCALAR = 1, FX_MUL_SCALAR = 2, FX_
                                   const T* bc);                                                                        \
     int fx_sgd_step_multi_##S(fx_ctx* ctx, int count, T* const* p, const T* const* g, const int64_t* n, T lr);         \
     int fx_sgd_momentum_step_multi_##S(fx_ctx* ctx, int count, T* const* p, const T* const* g, T* const* buf,          \
-                                       const int64_t* n, T lr, T momentum, T weight_decay, int nesterov);
+                                       const int64_t* n, T lr, T momentum, T weight_decay, int nesterov);               \
+    /* ---- a language model's training step ----  The reference trains image classifiers and has none of these; they sit\
+       beside its layers, losses and optimizers in the same form.  All tensors are dense, token ids are int64 on the device.\
+                                                                                                                       \
+       Embedding lookup and its weight gradient.  fwd: out[n, :] = scale * W[ids[n], :]; an id outside 0 .. vocab - 1  \
+       (padding) gives a row of zeros.  bwd: dW[v, :] = scale * the sum of g[n, :] over the n with ids[n] = v; every row of\
+       dW is written, rows of ids that do not occur with zeros, and tokens with an id outside the table count nowhere.  The\
+       sums run over the tokens sorted by id, in one order per ids array: no atomics, equal bits on every call. */     \
+    int fx_embedding_fwd_##S(fx_ctx* ctx, const T* W, const int64_t* ids, T* out, int64_t n, int64_t vocab, int64_t dim,\
+                             T scale);                                                                                 \
+    int fx_embedding_bwd_##S(fx_ctx* ctx, const T* g, const int64_t* ids, T* dW, int64_t n, int64_t vocab, int64_t dim,\
+                             T scale);                                                                                 \
+    /* Root-mean-square norm over the rows of [rows, dim], with the residual's addition in front of it.                \
+       fwd: h = x + res (res and h both NULL: h is x); rstd[row] = 1/sqrt(mean(h*h) + eps) (may be NULL); y = (h*rstd)*w.\
+       h may be x or res themselves and y may be x or res, but not both the same tensor.                               \
+       bwd, from the gradients dy of y and dh of h along the residual stream (dh may be NULL): dx = dh + rstd*(w*dy) - \
+       h*rstd^3*mean(w*dy*h), the gradient of x and of res alike; dw = the sum over rows of dy*(h*rstd) (dw may be NULL).\
+       dx may be dy or dh.  dw is summed in a fixed order per shape. */                                                \
+    int fx_rmsnorm_fwd_##S(fx_ctx* ctx, const T* x, const T* res, const T* w, double eps, T* h, T* y, T* rstd,         \
+                           int64_t rows, int64_t dim);                                                                 \
+    int fx_rmsnorm_bwd_##S(fx_ctx* ctx, const T* dy, const T* dh, const T* h, const T* w, const T* rstd, T* dx, T* dw, \
+                           int64_t rows, int64_t dim);                                                                 \
+    /* fx_gemm_bias_act with more in the product's store: pre = op(A).op(B) + bias[n] and C = act(pre) + residual, act \
+       0 none, 1 ReLU, 2 GELU (x*Phi(x)), 3 SiLU (x*sigmoid(x)).  bias [N], residual [M, N] and pre [M, N] (written, for\
+       the backward) may each be NULL.  Outputs share memory with nothing else. */                                     \
+    int fx_gemm_bias_act_residual_##S(fx_ctx* ctx, int trans_a, int trans_b, int64_t M, int64_t N, int64_t K, const T* A,\
+                                      const T* B, const T* bias, const T* residual, T* pre, T* C, int act);            \
+    /* Backward of the Linear layer Y[B, out] = act(X.W^T + b) + residual: dpre = dY*act'(pre) [B, out] (written; may be dY\
+       or pre themselves), dX[B, in] = dpre.W, dW[out, in] = dpre^T.X, db[out] = column sums of dpre (may be NULL).  The\
+       residual's gradient is dY.  dX and dW have the bits of fx_linear_bwd on dpre. */                                \
+    int fx_linear_act_bwd_##S(fx_ctx* ctx, int64_t B, int64_t in, int64_t out, const T* dY, const T* W, const T* X,    \
+                              const T* pre, int act, T* dpre, T* dX, T* dW, T* db);                                    \
+    /* Gated linear recurrence along the steps of [B, steps, dim]: f = sigmoid(z), h_t = f_t*h_{t-1} + (1 - f_t)*x_t with\
+       h_{-1} = h0 [B, dim] (NULL: 0).  The last step's h is the next segment's h0; steps = 1 is the generating form.  \
+       bwd, from dh [B, steps, dim] and dh_next [B, dim], the gradient that arrives at the last state from the next segment\
+       (its dh0; NULL: none): dz, dx [B, steps, dim] and dh0 [B, dim] (may be NULL), with h and h0 as in the forward call.\
+       Outputs share memory with nothing else. */                                                                      \
+    int fx_gated_recurrence_fwd_##S(fx_ctx* ctx, const T* z, const T* x, const T* h0, T* h, int64_t B, int64_t steps,  \
+                                    int64_t dim);                                                                      \
+    int fx_gated_recurrence_bwd_##S(fx_ctx* ctx, const T* dh, const T* z, const T* x, const T* h, const T* h0,         \
+                                    const T* dh_next, T* dz, T* dx, T* dh0, int64_t B, int64_t steps, int64_t dim);    \
+    /* The norm of all gradients together and their clipping by it, in front of fx_adam_step_multi / fx_sgd_step_multi with\
+       the same tables (HOST arrays of `count` device pointers / element counts): norm[0] (on the device) = sqrt of the sum\
+       of g*g over all tensors; clip: out[k] = g[k] * (norm > max_norm ? max_norm/norm : 1).  out[k] may be g[k] (nothing is\
+       written then where nothing is scaled), and shares memory with no other tensor of the call.  Squares are added in\
+       double for both types, in a fixed order.  A norm that is infinite or NaN scales nothing: the caller finds it in \
+       norm[0].  No host synchronisation: the calls may be recorded (fx_graph_*). */                                   \
+    int fx_grad_norm_multi_##S(fx_ctx* ctx, int count, const T* const* g, const int64_t* n, T* norm);                  \
+    int fx_clip_grad_norm_multi_##S(fx_ctx* ctx, int count, const T* const* g, T* const* out, const int64_t* n,        \
+                                    double max_norm, T* norm);
 
 FX_DECLARE_KERNELS(float, f32)
 FX_DECLARE_KERNELS(double, f64)

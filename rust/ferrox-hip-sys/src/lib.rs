@@ -203,6 +203,16 @@ extern "C" {
     pub fn fx_adam_step_multi_bc_f32(ctx: *mut fx_ctx, count: c_int, p: *const *mut f32, g: *const *const f32, m: *const *mut f32, v: *const *mut f32, vmax: *const *mut f32, n: *const i64, lr: f32, beta1: f32, beta2: f32, eps: f32, weight_decay: f32, bc: *const f32) -> c_int;
     pub fn fx_sgd_step_multi_f32(ctx: *mut fx_ctx, count: c_int, p: *const *mut f32, g: *const *const f32, n: *const i64, lr: f32) -> c_int;
     pub fn fx_sgd_momentum_step_multi_f32(ctx: *mut fx_ctx, count: c_int, p: *const *mut f32, g: *const *const f32, buf: *const *mut f32, n: *const i64, lr: f32, momentum: f32, weight_decay: f32, nesterov: c_int) -> c_int;
+    pub fn fx_embedding_fwd_f32(ctx: *mut fx_ctx, W: *const f32, ids: *const i64, out: *mut f32, n: i64, vocab: i64, dim: i64, scale: f32) -> c_int;
+    pub fn fx_embedding_bwd_f32(ctx: *mut fx_ctx, g: *const f32, ids: *const i64, dW: *mut f32, n: i64, vocab: i64, dim: i64, scale: f32) -> c_int;
+    pub fn fx_rmsnorm_fwd_f32(ctx: *mut fx_ctx, x: *const f32, res: *const f32, w: *const f32, eps: f64, h: *mut f32, y: *mut f32, rstd: *mut f32, rows: i64, dim: i64) -> c_int;
+    pub fn fx_rmsnorm_bwd_f32(ctx: *mut fx_ctx, dy: *const f32, dh: *const f32, h: *const f32, w: *const f32, rstd: *const f32, dx: *mut f32, dw: *mut f32, rows: i64, dim: i64) -> c_int;
+    pub fn fx_gemm_bias_act_residual_f32(ctx: *mut fx_ctx, trans_a: c_int, trans_b: c_int, M: i64, N: i64, K: i64, A: *const f32, B: *const f32, bias: *const f32, residual: *const f32, pre: *mut f32, C: *mut f32, act: c_int) -> c_int;
+    pub fn fx_linear_act_bwd_f32(ctx: *mut fx_ctx, B: i64, input: i64, out: i64, dY: *const f32, W: *const f32, X: *const f32, pre: *const f32, act: c_int, dpre: *mut f32, dX: *mut f32, dW: *mut f32, db: *mut f32) -> c_int;
+    pub fn fx_gated_recurrence_fwd_f32(ctx: *mut fx_ctx, z: *const f32, x: *const f32, h0: *const f32, h: *mut f32, B: i64, steps: i64, dim: i64) -> c_int;
+    pub fn fx_gated_recurrence_bwd_f32(ctx: *mut fx_ctx, dh: *const f32, z: *const f32, x: *const f32, h: *const f32, h0: *const f32, dh_next: *const f32, dz: *mut f32, dx: *mut f32, dh0: *mut f32, B: i64, steps: i64, dim: i64) -> c_int;
+    pub fn fx_grad_norm_multi_f32(ctx: *mut fx_ctx, count: c_int, g: *const *const f32, n: *const i64, norm: *mut f32) -> c_int;
+    pub fn fx_clip_grad_norm_multi_f32(ctx: *mut fx_ctx, count: c_int, g: *const *const f32, out: *const *mut f32, n: *const i64, max_norm: f64, norm: *mut f32) -> c_int;
     pub fn fx_fill_f64(ctx: *mut fx_ctx, out: *mut f64, value: f64, n: i64) -> c_int;
     pub fn fx_fill_uniform_f64(ctx: *mut fx_ctx, out: *mut f64, n: i64, seed: u64, lo: f64, hi: f64) -> c_int;
     pub fn fx_fill_normal_f64(ctx: *mut fx_ctx, out: *mut f64, n: i64, seed: u64, mean: f64, std: f64) -> c_int;
@@ -275,6 +285,16 @@ extern "C" {
     pub fn fx_adam_step_multi_bc_f64(ctx: *mut fx_ctx, count: c_int, p: *const *mut f64, g: *const *const f64, m: *const *mut f64, v: *const *mut f64, vmax: *const *mut f64, n: *const i64, lr: f64, beta1: f64, beta2: f64, eps: f64, weight_decay: f64, bc: *const f64) -> c_int;
     pub fn fx_sgd_step_multi_f64(ctx: *mut fx_ctx, count: c_int, p: *const *mut f64, g: *const *const f64, n: *const i64, lr: f64) -> c_int;
     pub fn fx_sgd_momentum_step_multi_f64(ctx: *mut fx_ctx, count: c_int, p: *const *mut f64, g: *const *const f64, buf: *const *mut f64, n: *const i64, lr: f64, momentum: f64, weight_decay: f64, nesterov: c_int) -> c_int;
+    pub fn fx_embedding_fwd_f64(ctx: *mut fx_ctx, W: *const f64, ids: *const i64, out: *mut f64, n: i64, vocab: i64, dim: i64, scale: f64) -> c_int;
+    pub fn fx_embedding_bwd_f64(ctx: *mut fx_ctx, g: *const f64, ids: *const i64, dW: *mut f64, n: i64, vocab: i64, dim: i64, scale: f64) -> c_int;
+    pub fn fx_rmsnorm_fwd_f64(ctx: *mut fx_ctx, x: *const f64, res: *const f64, w: *const f64, eps: f64, h: *mut f64, y: *mut f64, rstd: *mut f64, rows: i64, dim: i64) -> c_int;
+    pub fn fx_rmsnorm_bwd_f64(ctx: *mut fx_ctx, dy: *const f64, dh: *const f64, h: *const f64, w: *const f64, rstd: *const f64, dx: *mut f64, dw: *mut f64, rows: i64, dim: i64) -> c_int;
+    pub fn fx_gemm_bias_act_residual_f64(ctx: *mut fx_ctx, trans_a: c_int, trans_b: c_int, M: i64, N: i64, K: i64, A: *const f64, B: *const f64, bias: *const f64, residual: *const f64, pre: *mut f64, C: *mut f64, act: c_int) -> c_int;
+    pub fn fx_linear_act_bwd_f64(ctx: *mut fx_ctx, B: i64, input: i64, out: i64, dY: *const f64, W: *const f64, X: *const f64, pre: *const f64, act: c_int, dpre: *mut f64, dX: *mut f64, dW: *mut f64, db: *mut f64) -> c_int;
+    pub fn fx_gated_recurrence_fwd_f64(ctx: *mut fx_ctx, z: *const f64, x: *const f64, h0: *const f64, h: *mut f64, B: i64, steps: i64, dim: i64) -> c_int;
+    pub fn fx_gated_recurrence_bwd_f64(ctx: *mut fx_ctx, dh: *const f64, z: *const f64, x: *const f64, h: *const f64, h0: *const f64, dh_next: *const f64, dz: *mut f64, dx: *mut f64, dh0: *mut f64, B: i64, steps: i64, dim: i64) -> c_int;
+    pub fn fx_grad_norm_multi_f64(ctx: *mut fx_ctx, count: c_int, g: *const *const f64, n: *const i64, norm: *mut f64) -> c_int;
+    pub fn fx_clip_grad_norm_multi_f64(ctx: *mut fx_ctx, count: c_int, g: *const *const f64, out: *const *mut f64, n: *const i64, max_norm: f64, norm: *mut f64) -> c_int;
     pub fn fx_conv2d_last_path(ctx: *mut fx_ctx) -> *const c_char;
     pub fn fx_conv2d_bwd_relu_supported(ctx: *mut fx_ctx, kind: c_int, dtype: c_int, B: i64, Cin: i64, H: i64, W: i64, Cout: i64, kh: i64, kw: i64, sh: i64, sw: i64, ph: i64, pw: i64) -> c_int;
     pub fn fx_graph_begin(ctx: *mut fx_ctx) -> c_int;
