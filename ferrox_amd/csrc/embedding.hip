@@ -4,8 +4,10 @@
 //
 // The lookup is a gather of rows, bound by memory.  The gradient sorts the (id, n) pairs by id, stably, and then adds the rows of g
 // along the sorted order: every token's row is read once, no atomics, and the order of every sum depends on the ids alone.
-//   sort     up to 16384 tokens: one block, keys and positions in LDS; more: radix passes of 8 bits over tiles of 4096 tokens
-//            (counts per tile, one scan over digits and tiles, stable scatter).
+//   sort     up to 32768 tokens: one launch in which every block owns 256 consecutive ids, reads all tokens, keeps those of its ids
+//            in LDS and places them by one stable counting pass; how many tokens lie below its ids is counted on the way and is where
+//            its part of the order begins.  More tokens (or so many ids that the blocks would read too much): radix passes of 8 bits
+//            over tiles of 4096 tokens (counts per tile, one scan over digits and tiles, stable scatter).
 //   add      a piece of P consecutive sorted positions is summed by the threads of one (or a part of one) block, which run along
 //            the row; an id whose tokens all lie in one piece is written at once, an id that crosses a piece's border leaves one
 //            partial row per piece.  The same launch writes the zero rows of the ids that do not occur.
@@ -54,7 +56,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict_
 
 // ---- stable sort of the ids ------------------------------------------------------------------------------------------------------
 constexpr int SORT_NT = 1024, SORT_WAVES = SORT_NT / 64, BITS = 8, BINS = 1 << BITS;
-constexpr int SMALL_MAX = 16384, TILE = 4096;
+constexpr int RANGE_MAX = 32768, TILE = 4096;  // tokens: positions of the one-launch sort fit 16 bits and its LDS
 
 // padding sorts behind every id
 __device__ __forceinline__ uint32_t key_of(int64_t id, i64 vocab) { return id >= 0 && id < vocab ? (uint32_t)id : (uint32_t)vocab; }
@@ -115,48 +117,104 @@ __device__ __forceinline__ void scan_counts(uint32_t* counts, uint32_t* wsum) {
     __syncthreads();
 }
 
-// All passes in one block: K items per thread, n <= 1024 K.
+// The one-launch sort: block b owns ids 256 b .. 256 b + 255 (the last block also the padding key `vocab`), n <= 1024 K.
+// Reading: thread t of wave w holds tokens (w K + j) 64 + lane, all loads in flight at once.
 template <int K>
-__global__ __launch_bounds__(SORT_NT) void sort_small_kernel(const int64_t* __restrict__ ids, uint32_t* __restrict__ keys, uint32_t* __restrict__ pos, int n,
-                                                             i64 vocab, int passes) {
+__global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __restrict__ ids, uint32_t* __restrict__ keys, uint32_t* __restrict__ pos,
+                                                             int n, i64 vocab) {
     FX_DYNAMIC_SMEM(uint32_t, smem);
-    uint32_t* counts = smem;                       // [SORT_WAVES][BINS]
-    uint32_t* wsum = counts + SORT_WAVES * BINS;   // 4
-    uint32_t* kbuf = wsum + 4;                     // [K * SORT_NT]
-    uint16_t* pbuf = reinterpret_cast<uint16_t*>(kbuf + K * SORT_NT);
+    uint32_t* counts = smem;                                   // [SORT_WAVES][BINS]
+    uint32_t* start = counts + SORT_WAVES * BINS;              // [BINS]: where the next item of a digit goes
+    uint32_t* wsum = start + BINS;                             // 4
+    uint32_t* inside = wsum + 4;                               // [SORT_WAVES]: tokens of this block's ids per wave
+    uint32_t* below = inside + SORT_WAVES;                     // [SORT_WAVES]: tokens of smaller ids per wave
+    uint16_t* lpos = reinterpret_cast<uint16_t*>(below + SORT_WAVES);  // [K * SORT_NT]: the kept tokens, in order
+    uint8_t* ldig = reinterpret_cast<uint8_t*>(lpos + K * SORT_NT);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t key[K], at[K], rank[K];
+    const uint32_t lo = blockIdx.x * BINS;
+    uint32_t key[K];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
         const int i = (wave * K + j) * 64 + lane;
-        at[j] = i;
-        key[j] = i < n ? key_of(ids[i], vocab) : 0xffffffffu;  // behind everything in every pass
+        key[j] = i < n ? key_of(ids[i], vocab) : 0xffffffffu;
     }
-    for (int p = 0; p < passes; ++p) {
-        rank_items<K>(key, p * BITS, rank, counts);
-        scan_counts(counts, wsum);
+    uint32_t in = 0, lt = 0;
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const uint32_t to = counts[wave * BINS + ((key[j] >> (p * BITS)) & (BINS - 1))] + rank[j];
-            kbuf[to] = key[j];
-            pbuf[to] = (uint16_t)at[j];
+    for (int j = 0; j < K; ++j) {
+        in += (uint32_t)__popcll(__ballot(key[j] - lo < (uint32_t)BINS));
+        lt += (uint32_t)__popcll(__ballot(key[j] < lo));
+    }
+    if (lane == 0) {
+        inside[wave] = in;
+        below[wave] = lt;
+    }
+    if (threadIdx.x < BINS) start[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t at = 0, m = 0, base = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+        if (w < wave) at += inside[w];
+        m += inside[w];
+        base += below[w];
+    }
+    if (m == 0) return;  // block-uniform
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const uint32_t d = key[j] - lo;
+        const bool mine = d < (uint32_t)BINS;
+        const uint64_t who = __ballot(mine);
+        if (mine) {
+            const uint32_t to = at + (uint32_t)__popcll(who & ((1ull << lane) - 1));
+            lpos[to] = (uint16_t)((wave * K + j) * 64 + lane);
+            ldig[to] = (uint8_t)d;
+            atomicAdd(&start[d], 1u);  // whole numbers: any order
+        }
+        at += (uint32_t)__popcll(who);
+    }
+    __syncthreads();
+    // counts per digit -> where the digit begins
+    uint32_t sum = 0, incl = 0;
+    if (threadIdx.x < BINS) {
+        sum = incl = start[threadIdx.x];
+#pragma unroll
+        for (int q = 1; q < 64; q <<= 1) {
+            const uint32_t o = __shfl_up(incl, q, 64);
+            if (lane >= q) incl += o;
+        }
+        if (lane == 63) wsum[wave] = incl;
+    }
+    __syncthreads();
+    if (threadIdx.x < BINS) {
+        uint32_t s = base + incl - sum;
+        for (int w = 0; w < wave; ++w) s += wsum[w];
+        start[threadIdx.x] = s;
+    }
+    constexpr int R = K < 4 ? K : 4;  // items per thread and round
+    for (uint32_t r = 0; r < m; r += R * SORT_NT) {
+        uint32_t dig[R], rank[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const uint32_t i = r + (wave * R + j) * 64 + lane;
+            dig[j] = i < m ? ldig[i] : BINS - 1;  // past the list: behind every item of the last digit
+        }
+        rank_items<R>(dig, 0, rank, counts);
+        scan_counts(counts, wsum);
+        // counts[wave][d] - counts[0][d]: items of the digit in the waves in front
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const uint32_t i = r + (wave * R + j) * 64 + lane;
+            if (i < m) {
+                const uint32_t to = start[dig[j]] + counts[wave * BINS + dig[j]] - counts[dig[j]] + rank[j];
+                keys[to] = lo + dig[j];
+                pos[to] = lpos[i];
+            }
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const int i = (wave * K + j) * 64 + lane;
-            key[j] = kbuf[i];
-            at[j] = pbuf[i];
+        if (threadIdx.x < BINS) {  // the round's items of a digit: the distance to the next digit's start
+            const uint32_t d = threadIdx.x;
+            start[d] += (d + 1 < BINS ? counts[d + 1] : min(m - r, (uint32_t)(R * SORT_NT))) - counts[d];
         }
-        __syncthreads();  // before the next pass scatters over what was just read
-    }
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-        const int i = (wave * K + j) * 64 + lane;
-        if (i < n) {
-            keys[i] = key[j];
-            pos[i] = at[j];
-        }
+        __syncthreads();  // before the next round clears the counts
     }
 }
 
@@ -361,15 +419,18 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t* __r
     const i64 first = b * a.P;                                          // piece b's first position
     const bool whole = keys[first] == k;                                // the run holds all of piece b
     if (whole && first > 0 && keys[first - 1] == k) return;             // an earlier border has it
-    // last piece of the run: the piece of its last position
-    i64 lo = border, hi = a.n;
-    while (lo < hi) {
-        const i64 mid = (lo + hi) >> 1;
-        if (keys[mid] <= k) lo = mid + 1;
-        else hi = mid;
-    }
-    const i64 end = (lo - 1) / a.P;
+    // the run's last piece: the first from b + 1 on that is the last one or ends before the run does; 64 pieces are looked at together
     const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+    i64 end = b + 1;
+    for (;;) {
+        const i64 q = min(end + lane, (i64)a.pieces - 1);
+        const uint64_t stops = __ballot(q + 1 >= (i64)a.pieces || keys[(q + 1) * a.P] != k);
+        if (stops) {
+            end = min(end + __ffsll((unsigned long long)stops) - 1, (i64)a.pieces - 1);
+            break;
+        }
+        end += 64;
+    }
     const i64 col = ((i64)blockIdx.y * 64 + lane) * V;
     T acc[V];
 #pragma unroll
@@ -433,11 +494,11 @@ int embedding_fwd(fx_ctx* c, const T* W, const int64_t* ids, T* out, i64 n, i64 
     return FX_OK;
 }
 
-template <int K> int sort_small(fx_ctx* c, const int64_t* ids, uint32_t* keys, uint32_t* pos, i64 n, i64 vocab, int passes) {
-    constexpr size_t lds = (SORT_WAVES * BINS + 4) * 4 + (size_t)K * SORT_NT * 6;
-    static const hipError_t attr = hipFuncSetAttribute((const void*)sort_small_kernel<K>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+template <int K> int sort_range(fx_ctx* c, const int64_t* ids, uint32_t* keys, uint32_t* pos, i64 n, i64 vocab) {
+    constexpr size_t lds = (SORT_WAVES * BINS + BINS + 4 + 2 * SORT_WAVES) * 4 + (size_t)K * SORT_NT * 3;
+    static const hipError_t attr = hipFuncSetAttribute((const void*)sort_range_kernel<K>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     FX_HIP_CHECK(attr);
-    FX_LAUNCH(dim3(1), dim3(SORT_NT), lds, c->stream, (ids, keys, pos, (int)n, vocab, passes), sort_small_kernel<K>);
+    FX_LAUNCH(dim3((unsigned)(vocab / BINS + 1)), dim3(SORT_NT), lds, c->stream, (ids, keys, pos, (int)n, vocab), sort_range_kernel<K>);
     FX_LAUNCH_CHECK();
     return FX_OK;
 }
@@ -477,7 +538,9 @@ int embedding_bwd(fx_ctx* c, const T* g, const int64_t* ids, T* dW, i64 n, i64 v
     a.tpp_log = 0;
     int passes = 1;
     while (passes < 4 && (vocab >> (BITS * passes)) != 0) ++passes;  // the largest key is vocab itself
-    const bool small = n <= SMALL_MAX;
+    // the one-launch sort while the blocks' reading of all tokens, 8 bytes each, stays below 128 MB (about 15 us from the L2s): up to
+    // 32768 tokens of 131000 ids, 4096 of a million
+    const bool small = n <= RANGE_MAX && n * (vocab / BINS + 1) <= (1ll << 24);
     const i64 tiles = fx::ceil_div(n, (i64)TILE), entries = tiles * BINS;
     // scratch: [keys][pos] once or twice, the table of counts, the partial rows
     const i64 nkeys = fx::ceil_div(n, (i64)64) * 64, lists = small ? 2 : 4;
@@ -488,9 +551,10 @@ int embedding_bwd(fx_ctx* c, const T* g, const int64_t* ids, T* dW, i64 n, i64 v
     uint32_t *keys = lists_p, *pos = lists_p + nkeys;
     if (n > 0 && small) {
         int rc;
-        if (n <= SORT_NT) rc = sort_small<1>(c, ids, keys, pos, n, vocab, passes);
-        else if (n <= 4 * SORT_NT) rc = sort_small<4>(c, ids, keys, pos, n, vocab, passes);
-        else rc = sort_small<16>(c, ids, keys, pos, n, vocab, passes);
+        if (n <= SORT_NT) rc = sort_range<1>(c, ids, keys, pos, n, vocab);
+        else if (n <= 4 * SORT_NT) rc = sort_range<4>(c, ids, keys, pos, n, vocab);
+        else if (n <= 16 * SORT_NT) rc = sort_range<16>(c, ids, keys, pos, n, vocab);
+        else rc = sort_range<32>(c, ids, keys, pos, n, vocab);
         if (rc) return rc;
     } else if (n > 0) {
         uint32_t* table = lists_p + 4 * nkeys;

@@ -3,8 +3,8 @@
 //   backward:  dx_j = dh_j + rstd (w_j dy_j) - h_j rstd^3 (sum_k w_k dy_k h_k) / D;  dw_j = sum over rows of dy_j (h_j rstd)
 // Both are bound by memory: 2 reads and 2 writes of [rows, D] forward, 3 reads and 1 write backward.  A row stays in registers
 // between its one read and its one write: up to 16 elements per thread, one wave per row up to 1024 elements, a block of 256 up to
-// 4096 and of 1024 up to 16384; longer rows are read twice.  Rows that are not whole aligned 16-byte vectors are read element by
-// element.  Sums are held in the tensors' own type (f32 or f64): a thread adds at most 16 terms before the tree of its block.
+// 4096 and of 1024 up to 16384; longer rows are read twice.  All accesses are 16-byte vectors that start at any element (a row of an
+// odd length moves the next one off the 16-byte grid); only the last, incomplete vector of a row goes element by element.  Sums are held in the tensors' own type (f32 or f64): a thread adds at most 16 terms before the tree of its block.
 // The weight gradient is added up in registers over the rows that a block takes (thread t owns the same columns in every row), one
 // partial row per block, and the partial rows are added by a second launch in a fixed order: no atomics.
 #include <mutex>
@@ -33,30 +33,16 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_fwd_kernel(const T* x, c
     T v[NV][V];
     T s = T(0);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int j = (k * NT + t) * V;
-        if (j < D) {
-            load<V>(x + base + j, v[k]);
-        } else {
-#pragma unroll
-            for (int u = 0; u < V; ++u) v[k][u] = T(0);
-        }
-    }
+    for (int k = 0; k < NV; ++k) load_part<V>(x + base, (k * NT + t) * V, D, v[k]);
     if constexpr (RES) {
         T r[NV][V];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int j = (k * NT + t) * V;
-            if (j < D) load<V>(res + base + j, r[k]);
-        }
+        for (int k = 0; k < NV; ++k) load_part<V>(res + base, (k * NT + t) * V, D, r[k]);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int j = (k * NT + t) * V;
-            if (j < D) {
 #pragma unroll
-                for (int u = 0; u < V; ++u) v[k][u] = v[k][u] + r[k][u];
-                store<V>(h + base + j, v[k]);
-            }
+            for (int u = 0; u < V; ++u) v[k][u] = v[k][u] + r[k][u];
+            store_part<V>(h + base, (k * NT + t) * V, D, v[k]);
         }
     }
 #pragma unroll
@@ -68,14 +54,11 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_fwd_kernel(const T* x, c
     if (t == 0 && rstd) rstd[row] = r;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int j = (k * NT + t) * V;
-        if (j < D) {
-            T g[V];
-            load<V>(w + j, g);
+        T g[V];
+        load_part<V>(w, (k * NT + t) * V, D, g);
 #pragma unroll
-            for (int u = 0; u < V; ++u) g[u] = (v[k][u] * r) * g[u];
-            store<V>(y + base + j, g);
-        }
+        for (int u = 0; u < V; ++u) g[u] = (v[k][u] * r) * g[u];
+        store_part<V>(y + base, (k * NT + t) * V, D, g);
     }
 }
 
@@ -151,8 +134,7 @@ int rmsnorm_fwd(fx_ctx* c, const T* x, const T* res, const T* w, double eps, T* 
         FX_LAUNCH_CHECK();
         return FX_OK;
     }
-    const bool vec = D % V == 0 && fx::aligned16(x) && fx::aligned16(w) && fx::aligned16(y) && (!res || (fx::aligned16(res) && fx::aligned16(h)));
-    return vec ? dispatch_fwd<T, V>(c, x, res, w, e, h, y, rstd, rows, D) : dispatch_fwd<T, 1>(c, x, res, w, e, h, y, rstd, rows, D);
+    return dispatch_fwd<T, V>(c, x, res, w, e, h, y, rstd, rows, D);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------
@@ -167,10 +149,9 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_bwd_kernel(const T* dy, 
     T wv[NV][V], dw[NV][V];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int j = (k * NT + t) * V;
 #pragma unroll
-        for (int u = 0; u < V; ++u) dw[k][u] = wv[k][u] = T(0);
-        if (j < D) load<V>(w + j, wv[k]);
+        for (int u = 0; u < V; ++u) dw[k][u] = T(0);
+        load_part<V>(w, (k * NT + t) * V, D, wv[k]);
     }
     for (i64 row = (i64)blockIdx.x * GR + group; row < rows; row += (i64)gridDim.x * GR) {
         const i64 base = row * D;
@@ -178,14 +159,8 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_bwd_kernel(const T* dy, 
         T g[NV][V], hv[NV][V];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int j = (k * NT + t) * V;
-            if (j < D) {
-                load<V>(dy + base + j, g[k]);
-                load<V>(h + base + j, hv[k]);
-            } else {
-#pragma unroll
-                for (int u = 0; u < V; ++u) g[k][u] = hv[k][u] = T(0);
-            }
+            load_part<V>(dy + base, (k * NT + t) * V, D, g[k]);
+            load_part<V>(h + base, (k * NT + t) * V, D, hv[k]);
         }
         T s = T(0);
 #pragma unroll
@@ -201,17 +176,14 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_bwd_kernel(const T* dy, 
         const T q = (s / T(D)) * (r * r);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int j = (k * NT + t) * V;
-            if (j < D) {
-                T d[V];
-                if (dh) load<V>(dh + base + j, d);
+            T d[V];
+            if (dh) load_part<V>(dh + base, (k * NT + t) * V, D, d);
 #pragma unroll
-                for (int u = 0; u < V; ++u) {
-                    const T a = r * (g[k][u] - hv[k][u] * q);
-                    d[u] = dh ? a + d[u] : a;
-                }
-                store<V>(dx + base + j, d);
+            for (int u = 0; u < V; ++u) {
+                const T a = r * (g[k][u] - hv[k][u] * q);
+                d[u] = dh ? a + d[u] : a;
             }
+            store_part<V>(dx + base, (k * NT + t) * V, D, d);
         }
     }
     if (!part) return;
@@ -229,10 +201,7 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_bwd_kernel(const T* dy, 
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int j = (k * NT + t) * V;
-            if (j < D) store<V>(part + (i64)blockIdx.x * D + j, dw[k]);
-        }
+        for (int k = 0; k < NV; ++k) store_part<V>(part + (i64)blockIdx.x * D, (k * NT + t) * V, D, dw[k]);
     }
 }
 
@@ -322,9 +291,7 @@ int rmsnorm_bwd(fx_ctx* c, const T* dy, const T* dh, const T* h, const T* w, con
         FX_LAUNCH_CHECK();
         return FX_OK;
     }
-    const bool vec = D % V == 0 && fx::aligned16(dy) && fx::aligned16(h) && fx::aligned16(w) && fx::aligned16(dx) && (!dh || fx::aligned16(dh)) &&
-                     (!dw || fx::aligned16(dw));
-    return vec ? dispatch_bwd<T, V>(c, dy, dh, h, w, rstd, dx, dw, rows, D) : dispatch_bwd<T, 1>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
+    return dispatch_bwd<T, V>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
 }
 }  // namespace
 

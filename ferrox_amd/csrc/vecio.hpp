@@ -5,7 +5,8 @@
 
 namespace vio {
 
-template <typename T, int V> struct VecOf { typedef T type __attribute__((ext_vector_type(V))); };
+// Element-aligned: the GPU's 16-byte global accesses may start at any element, so a row need not begin on a 16-byte border.
+template <typename T, int V> struct VecOf { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T, int V> using Vec = typename VecOf<T, V>::type;
 
 template <int V, typename T> __device__ __forceinline__ void load(const T* p, T (&v)[V]) {
@@ -18,6 +19,28 @@ template <int V, typename T> __device__ __forceinline__ void store(T* p, const T
 #pragma unroll
     for (int u = 0; u < V; ++u) q[u] = v[u];
     *reinterpret_cast<Vec<T, V>*>(p) = q;
+}
+
+// The vector at column j of a row that ends at D: whole, or what is left of the row (the rest zero / not stored).
+template <int V, typename T> __device__ __forceinline__ void load_part(const T* row, int j, int D, T (&v)[V]) {
+    if (j + V <= D) {
+        load<V>(row + j, v);
+    } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            v[u] = T(0);
+            if (j + u < D) v[u] = row[j + u];
+        }
+    }
+}
+template <int V, typename T> __device__ __forceinline__ void store_part(T* row, int j, int D, const T (&v)[V]) {
+    if (j + V <= D) {
+        store<V>(row + j, v);
+    } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+            if (j + u < D) row[j + u] = v[u];
+    }
 }
 
 template <typename T> __device__ __forceinline__ T wave_sum(T v) {  // every lane gets the sum, in one fixed tree
