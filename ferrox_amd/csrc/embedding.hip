@@ -93,12 +93,15 @@ __device__ __forceinline__ void rank_items(const uint32_t (&key)[K], int shift, 
 __device__ __forceinline__ void scan_counts(uint32_t* counts, uint32_t* wsum) {
     __syncthreads();
     const int t = threadIdx.x, lane = t & 63;
-    uint32_t sum = 0, incl = 0;
+    uint32_t sum = 0, incl = 0, before[SORT_WAVES];
     if (t < BINS) {
+        uint32_t v[SORT_WAVES];  // all reads in flight before the first write
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) v[w] = counts[w * BINS + t];
+#pragma unroll
         for (int w = 0; w < SORT_WAVES; ++w) {
-            const uint32_t v = counts[w * BINS + t];
-            counts[w * BINS + t] = sum;
-            sum += v;
+            before[w] = sum;
+            sum += v[w];
         }
         incl = sum;
 #pragma unroll
@@ -112,7 +115,8 @@ __device__ __forceinline__ void scan_counts(uint32_t* counts, uint32_t* wsum) {
     if (t < BINS) {
         uint32_t base = incl - sum;
         for (int w = 0; w < (t >> 6); ++w) base += wsum[w];
-        for (int w = 0; w < SORT_WAVES; ++w) counts[w * BINS + t] += base;
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) counts[w * BINS + t] = base + before[w];
     }
     __syncthreads();
 }
@@ -130,6 +134,8 @@ __global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __re
     uint32_t* below = inside + SORT_WAVES;                     // [SORT_WAVES]: tokens of smaller ids per wave
     uint16_t* lpos = reinterpret_cast<uint16_t*>(below + SORT_WAVES);  // [K * SORT_NT]: the kept tokens, in order
     uint8_t* ldig = reinterpret_cast<uint8_t*>(lpos + K * SORT_NT);
+    constexpr int R = K < 4 ? K : 4;  // kept tokens per thread and round
+    constexpr uint32_t ROUND = R * SORT_NT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t lo = blockIdx.x * BINS;
     uint32_t key[K];
@@ -167,30 +173,31 @@ __global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __re
             const uint32_t to = at + (uint32_t)__popcll(who & ((1ull << lane) - 1));
             lpos[to] = (uint16_t)((wave * K + j) * 64 + lane);
             ldig[to] = (uint8_t)d;
-            atomicAdd(&start[d], 1u);  // whole numbers: any order
+            if (m > ROUND) atomicAdd(&start[d], 1u);  // whole numbers: any order
         }
         at += (uint32_t)__popcll(who);
     }
     __syncthreads();
-    // counts per digit -> where the digit begins
-    uint32_t sum = 0, incl = 0;
-    if (threadIdx.x < BINS) {
-        sum = incl = start[threadIdx.x];
+    // where each digit begins: with one round its own scan says it, with more of them the digits were counted above
+    if (m > ROUND) {  // block-uniform
+        uint32_t sum = 0, incl = 0;
+        if (threadIdx.x < BINS) {
+            sum = incl = start[threadIdx.x];
 #pragma unroll
-        for (int q = 1; q < 64; q <<= 1) {
-            const uint32_t o = __shfl_up(incl, q, 64);
-            if (lane >= q) incl += o;
+            for (int q = 1; q < 64; q <<= 1) {
+                const uint32_t o = __shfl_up(incl, q, 64);
+                if (lane >= q) incl += o;
+            }
+            if (lane == 63) wsum[wave] = incl;
         }
-        if (lane == 63) wsum[wave] = incl;
+        __syncthreads();
+        if (threadIdx.x < BINS) {
+            uint32_t s = base + incl - sum;
+            for (int w = 0; w < wave; ++w) s += wsum[w];
+            start[threadIdx.x] = s;
+        }
     }
-    __syncthreads();
-    if (threadIdx.x < BINS) {
-        uint32_t s = base + incl - sum;
-        for (int w = 0; w < wave; ++w) s += wsum[w];
-        start[threadIdx.x] = s;
-    }
-    constexpr int R = K < 4 ? K : 4;  // items per thread and round
-    for (uint32_t r = 0; r < m; r += R * SORT_NT) {
+    for (uint32_t r = 0; r < m; r += ROUND) {
         uint32_t dig[R], rank[R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -204,15 +211,17 @@ __global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __re
         for (int j = 0; j < R; ++j) {
             const uint32_t i = r + (wave * R + j) * 64 + lane;
             if (i < m) {
-                const uint32_t to = start[dig[j]] + counts[wave * BINS + dig[j]] - counts[dig[j]] + rank[j];
+                const uint32_t first = m > ROUND ? start[dig[j]] - counts[dig[j]] : base;
+                const uint32_t to = first + counts[wave * BINS + dig[j]] + rank[j];
                 keys[to] = lo + dig[j];
                 pos[to] = lpos[i];
             }
         }
+        if (m <= ROUND) return;
         __syncthreads();
         if (threadIdx.x < BINS) {  // the round's items of a digit: the distance to the next digit's start
             const uint32_t d = threadIdx.x;
-            start[d] += (d + 1 < BINS ? counts[d + 1] : min(m - r, (uint32_t)(R * SORT_NT))) - counts[d];
+            start[d] += (d + 1 < BINS ? counts[d + 1] : min(m - r, ROUND)) - counts[d];
         }
         __syncthreads();  // before the next round clears the counts
     }

@@ -27,7 +27,7 @@ typedef Tile<128, 128, 16, 64, 64> TileBig;    // 4 waves, 64x64 each
 typedef Tile<64, 64, 16, 32, 32> TileSmall;    // 4 waves, 32x32 each
 
 template <typename T, class Cfg, bool TA, bool TB>
-int run(fx_ctx* c, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* bias, int relu, bool* bias_pending) {
+int run(fx_ctx* c, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* bias, int relu, const gep::Epilogue<T>& ex, bool* bias_pending) {
     // A stored [M,K] (k contiguous) unless TA ([K,M], m contiguous); B stored [K,N] (n contiguous) unless TB ([N,K]).
     MatLoader<T, !TA> al{A, TA ? M : K, (int)M};
     MatLoader<T, TB> bl{B, TB ? K : N, (int)N};
@@ -39,53 +39,64 @@ int run(fx_ctx* c, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* b
             MatStore<T, true> ep{C, N, 0, (int)M, (int)N, bias, relu};
             return launch<T, Cfg>(c, al, bl, ep, M, N, K, 1, kps);
         }
+        if (ex.any()) {
+            if (gep::TileStore<T>::takes(ex.act)) {
+                gep::TileStore<T> ep{C, N, (int)M, (int)N, ex};
+                return launch<T, Cfg>(c, al, bl, ep, M, N, K, 1, kps);
+            }
+            *bias_pending = true;
+        }
         MatStore<T> ep{C, N, 0, (int)M, (int)N};
         return launch<T, Cfg>(c, al, bl, ep, M, N, K, 1, kps);
     }
     // split-K: the bias (and ReLU) ride in the ordered sum's store where its indices fit 32 bits, else the caller adds them after it
-    const bool in_sum = bias != nullptr && M * N <= 0x7fffffff;
-    *bias_pending = bias != nullptr && !in_sum;
+    const bool in_sum = (bias != nullptr || ex.any()) && M * N <= 0x7fffffff;
+    *bias_pending = (bias != nullptr || ex.any()) && !in_sum;
     T* part = (T*)c->get_scratch((i64)splits * M * N * (i64)sizeof(T));
     if (!part) return FX_ERR_OOM;
     MatStore<T> ep{part, N, M * N, (int)M, (int)N};
     if (int rc = launch<T, Cfg>(c, al, bl, ep, M, N, K, splits, kps)) return rc;
+    if (in_sum && ex.any()) return gep::launch_sum<T>(c, part, C, M, N, splits, ex);
     return launch_splitk_reduce<T>(c, part, C, M * N, splits, in_sum ? bias : nullptr, N, relu);
 }
 
 template <typename T, class Cfg>
-int run_trans(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* bias, int relu, bool* pend) {
-    if (!ta && !tb) return run<T, Cfg, false, false>(c, M, N, K, A, B, C, bias, relu, pend);
-    if (!ta && tb) return run<T, Cfg, false, true>(c, M, N, K, A, B, C, bias, relu, pend);
-    if (ta && !tb) return run<T, Cfg, true, false>(c, M, N, K, A, B, C, bias, relu, pend);
-    return run<T, Cfg, true, true>(c, M, N, K, A, B, C, bias, relu, pend);
+int run_trans(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* bias, int relu, const gep::Epilogue<T>& ex,
+              bool* pend) {
+    if (!ta && !tb) return run<T, Cfg, false, false>(c, M, N, K, A, B, C, bias, relu, ex, pend);
+    if (!ta && tb) return run<T, Cfg, false, true>(c, M, N, K, A, B, C, bias, relu, ex, pend);
+    if (ta && !tb) return run<T, Cfg, true, false>(c, M, N, K, A, B, C, bias, relu, ex, pend);
+    return run<T, Cfg, true, true>(c, M, N, K, A, B, C, bias, relu, ex, pend);
 }
 
 // the one-launch small-product kernel; with K split over blocks, its partial results and their ordered sum (bias and ReLU in the sum's store)
 int small_launch(fx_ctx* c, const gsmall::Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K, const float* A, const float* B, float* C, const float* bias,
-                 int relu, float* part, float* asum) {
-    return gsmall::run(c, pl, ta, tb, M, N, K, A, B, C, bias, relu, part, asum);
+                 int relu, float* part, float* asum, const gep::Epilogue<float>& ex) {
+    return gsmall::run(c, pl, ta, tb, M, N, K, A, B, C, bias, relu, part, asum, ex);
 }
 int small_launch(fx_ctx* c, const gsmall::Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K, const double* A, const double* B, double* C,
-                 const double* bias, int relu, double* part, double* asum) {
-    return gsmall::run_f64(c, pl, ta, tb, M, N, K, A, B, C, bias, relu, part, asum);
+                 const double* bias, int relu, double* part, double* asum, const gep::Epilogue<double>& ex) {
+    return gsmall::run_f64(c, pl, ta, tb, M, N, K, A, B, C, bias, relu, part, asum, ex);
 }
 // asum (optional, only with an unsplit reduction): the row sums of op(A) from the same launch
 template <typename T>
 int small_product(fx_ctx* c, const gsmall::Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* bias, int relu,
-                  T* asum = nullptr) {
+                  const gep::Epilogue<T>& ex, T* asum = nullptr) {
     T* part = nullptr;
     if (pl.splits > 1) {
         part = (T*)c->get_scratch(gsmall::workspace_bytes<T>(pl, M, N));
         if (!part) return FX_ERR_OOM;
     }
-    if (int rc = small_launch(c, pl, ta, tb, M, N, K, A, B, C, bias, relu, part, asum)) return rc;
+    if (int rc = small_launch(c, pl, ta, tb, M, N, K, A, B, C, bias, relu, part, asum, ex)) return rc;
+    if (pl.splits > 1 && ex.any()) return gep::launch_sum<T>(c, part, C, M, N, pl.splits, ex);
     return pl.splits > 1 ? launch_splitk_reduce<T>(c, part, C, M * N, pl.splits, bias, N, relu) : FX_OK;
 }
 
-// asum_done (optional): with asum != null, set when the launch that computed C also wrote asum[m] = sum over k of op(A)[m][k]
+// ex (in place of bias and relu): bias, activation, residual and pre in the product's store where its kernel takes them, else as a
+// pass of its own.  asum_done (optional): with asum != null, set when the launch that computed C also wrote asum[m] = sum over k of op(A)[m][k]
 template <typename T>
 int gemm(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B, T* C, const T* bias = nullptr, int relu = 0, T* asum = nullptr,
-         bool* asum_done = nullptr) {
+         bool* asum_done = nullptr, const gep::Epilogue<T>& ex = gep::Epilogue<T>()) {
     FX_CHECK_CTX(c);
     FX_REQUIRE(M >= 0 && N >= 0 && K >= 0, "fx_gemm: negative dimension");
     if (M == 0 || N == 0) return FX_OK;
@@ -102,17 +113,18 @@ int gemm(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B,
             static const bool generic_only = std::getenv("FX_GEMM_GENERIC") != nullptr;  // A/B timing switch
             const glk::Plan pl = glk::make_plan(c->num_cus, ta != 0, tb != 0, M, N, K, ta ? M : K, tb ? K : N);
             lds_path = pl.ok && !generic_only && fx::aligned16(A) && fx::aligned16(B) && fx::aligned16(C);
-            if (lds_path) rc = glk::run(c, pl, ta != 0, tb != 0, M, N, K, A, B, C, bias, relu);
+            if (lds_path) rc = glk::run(c, pl, ta != 0, tb != 0, M, N, K, A, B, C, bias, relu, 1, 0, 0, 0, 0, ex);
             else if (!generic_only && gthin::eligible(c->num_cus, ta != 0, tb != 0, M, N, K)) {
                 lds_path = true;
                 rc = gthin::run(c, M, N, K, A, B, C, bias, relu, asum);
+                pending = ex.any();
                 if (asum) *asum_done = true;
             } else if (!generic_only) {
                 const gsmall::Plan sp = gsmall::make_plan<float>(c->num_cus, ta != 0, tb != 0, M, N, K, A, B, asum == nullptr);
                 if (sp.ok) {
                     lds_path = true;
                     const bool with_sum = asum != nullptr && sp.splits == 1;
-                    rc = small_product<float>(c, sp, ta != 0, tb != 0, M, N, K, A, B, C, bias, relu, with_sum ? asum : nullptr);
+                    rc = small_product<float>(c, sp, ta != 0, tb != 0, M, N, K, A, B, C, bias, relu, ex, with_sum ? asum : nullptr);
                     if (with_sum) *asum_done = true;
                 }
             }
@@ -124,7 +136,7 @@ int gemm(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B,
                 if (sp.ok) {
                     lds_path = true;
                     const bool with_sum = asum != nullptr && sp.splits == 1;
-                    rc = small_product<double>(c, sp, ta != 0, tb != 0, M, N, K, A, B, C, bias, relu, with_sum ? asum : nullptr);
+                    rc = small_product<double>(c, sp, ta != 0, tb != 0, M, N, K, A, B, C, bias, relu, ex, with_sum ? asum : nullptr);
                     if (with_sum) *asum_done = true;
                 }
             }
@@ -132,10 +144,11 @@ int gemm(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const T* A, const T* B,
         if (lds_path) {
         } else if (K == 0) {  // empty sum
             rc = launch_zero<T>(c, C, M * N);
-            pending = bias != nullptr;
-        } else if (M >= 128 && N >= 128) rc = run_trans<T, TileBig>(c, ta, tb, M, N, K, A, B, C, bias, relu, &pending);
-        else rc = run_trans<T, TileSmall>(c, ta, tb, M, N, K, A, B, C, bias, relu, &pending);
+            pending = bias != nullptr || ex.any();
+        } else if (M >= 128 && N >= 128) rc = run_trans<T, TileBig>(c, ta, tb, M, N, K, A, B, C, bias, relu, ex, &pending);
+        else rc = run_trans<T, TileSmall>(c, ta, tb, M, N, K, A, B, C, bias, relu, ex, &pending);
         if (rc) return rc;
+        if (pending && ex.any()) return gep::launch_pass<T>(c, C, M * N, N, ex);
     }
     return pending ? bias_act_t(c, C, bias, M, N, relu) : FX_OK;
 }
@@ -231,16 +244,15 @@ int gemm_bias_act_residual(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const
                    !fx::overlap<T>(C, n, pre, n) && !fx::overlap<T>(pre, n, A, M * K) && !fx::overlap<T>(pre, n, B, K * N) &&
                    !fx::overlap<T>(pre, n, bias, N) && !fx::overlap<T>(pre, n, residual, n),
                "fx_gemm_bias_act_residual: an output overlaps another tensor of the call");
+    const gep::Epilogue<T> ex{bias, residual, pre, act};
     if (K == 0) {  // the empty product
         std::lock_guard<std::mutex> lk(c->launch_mutex);
         if (int rc = launch_zero<T>(c, C, n)) return rc;
-    } else if (int rc = gemm<T>(c, ta, tb, M, N, K, A, B, C)) {
-        return rc;
+        return ex.any() ? gep::launch_pass<T>(c, C, n, N, ex) : FX_OK;
     }
-    const gep::Epilogue<T> ep{bias, residual, pre, act};
-    if (!ep.any()) return FX_OK;
-    std::lock_guard<std::mutex> lk(c->launch_mutex);
-    return gep::launch_pass<T>(c, C, n, N, ep);
+    // what fx_gemm_bias_act does already goes its way, same kernels and bits
+    if (bias && !residual && !pre && act <= fxact::RELU) return gemm<T>(c, ta, tb, M, N, K, A, B, C, bias, act);
+    return gemm<T>(c, ta, tb, M, N, K, A, B, C, nullptr, 0, nullptr, nullptr, ex);
 }
 extern "C" int fx_gemm_bias_act_residual_f32(fx_ctx* c, int ta, int tb, int64_t M, int64_t N, int64_t K, const float* A, const float* B,
                                              const float* bias, const float* residual, float* pre, float* C, int act) {

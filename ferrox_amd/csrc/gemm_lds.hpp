@@ -18,7 +18,7 @@
 // Workgroup ids are handed to the eight XCDs round-robin by the hardware; the id -> tile map gives each XCD a
 // contiguous range of tiles so that the tiles resident on one XCD share operand panels in its L2.
 #pragma once
-#include "igemm_core.hpp"
+#include "gemm_epilogue.hpp"
 
 namespace glk {
 using igemm::f32x16;
@@ -41,12 +41,14 @@ struct Params {
     // a batch of independent products of one shape in one launch (blockIdx.y): element strides between them (0: shared operand)
     i64 sa = 0, sb = 0, sc = 0;
     int bias_per_row = 0;  // the bias belongs to the rows of C (a convolution's output channels) instead of its columns
+    gep::Epilogue<float> ex;  // EP == EP_FULL
 };
+constexpr int EP_NONE = 0, EP_BIAS = 1, EP_FULL = 2;  // what the store does: nothing, bias (+ ReLU), the whole of gep::Epilogue
 
 // TA: A is stored [K, M] (m contiguous); TB: B is stored [N, K] (k contiguous).
 // KT (both operands k-contiguous only): K need not be a multiple of the stage depth -- the last stage loads what is left of the rows
 // (K a multiple of 4: a 16-byte vector is inside a row or past it) and parks zeros behind it.
-template <int TN, int WM, bool TA, bool TB, bool BIAS, bool KT = false>
+template <int TN, int WM, bool TA, bool TB, int EP, bool KT = false>
 __global__ __launch_bounds__(NT, 2) void gemm_lds_kernel(const Params p) {
     static_assert(!KT || (!TA && TB), "the K tail is handled for k-contiguous operands");
     constexpr int WN = 4 / WM, BM = 32 * WM, BN = 32 * TN * WN;
@@ -252,6 +254,70 @@ __global__ __launch_bounds__(NT, 2) void gemm_lds_kernel(const Params p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[0][e] = acc[0][e] + acc[1][e];
     }
+    if constexpr (EP == EP_FULL) {
+        // Each wave turns its 32 rows through LDS (its own piece; every wave has left the slabs through the barrier that ended the
+        // last stage), 16-byte groups along a row then, so that bias, residual, pre and C move in 16-byte accesses and the
+        // activation is compiled for four elements instead of 16 TN.  Measured at 4096 x 1024 x 4096 with bias and residual: see gemm.hip.
+        constexpr int WC = 32 * TN, CG = WC / 4, RPI = 64 / CG;  // columns of the wave, groups per row, rows per pass
+        float* const turn = smem + wave * (32 * WC);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) turn[igemm::Mfma<float>::row(e, lane) * WC + j * 32 + l32] = acc[j][e];
+        __syncthreads();
+        const int n = n0 + wn * WC + 4 * (lane % CG), left = p.N - n;
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.ex.bias) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q < left) bias[q] = p.ex.bias[n + q];
+        }
+#pragma unroll 1
+        for (int r = lane / CG; r < 32; r += RPI) {
+            const int m = m0 + wm * 32 + r;
+            if (m >= p.M || left <= 0) continue;
+            const i64 i = (i64)m * p.N + n;
+            const float4 t4 = *reinterpret_cast<const float4*>(turn + r * WC + 4 * (lane % CG));
+            float v[4] = {t4.x, t4.y, t4.z, t4.w}, res[4] = {0.f, 0.f, 0.f, 0.f};
+            typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // a row of C starts at any element
+            if (p.ex.residual) {
+                if (left >= 4) {
+                    const f4u q4 = *reinterpret_cast<const f4u*>(p.ex.residual + i);
+                    res[0] = q4.x; res[1] = q4.y; res[2] = q4.z; res[3] = q4.w;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        if (q < left) res[q] = p.ex.residual[i + q];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (p.ex.bias) v[q] = v[q] + bias[q];
+            if (p.ex.pre) {
+                if (left >= 4) {
+                    *reinterpret_cast<f4u*>(p.ex.pre + i) = f4u{v[0], v[1], v[2], v[3]};
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        if (q < left) p.ex.pre[i + q] = v[q];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[q] = fxact::apply<float>(p.ex.act, v[q]);
+                if (p.ex.residual) v[q] = v[q] + res[q];
+            }
+            if (left >= 4) {
+                *reinterpret_cast<f4u*>(Cb + i) = f4u{v[0], v[1], v[2], v[3]};
+            } else {
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+                    if (q < left) Cb[i + q] = v[q];
+            }
+        }
+        return;
+    }
+    constexpr bool BIAS = EP == EP_BIAS;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
         const int n = n0 + (wn * TN + j) * 32 + l32;
@@ -327,14 +393,20 @@ inline int launch(fx_ctx* c, const Plan& pl, const Params& p, int batch) {
     if constexpr (!KT && !TA && TB) {
         if (p.K % KC != 0) return launch<TN, WM, TA, TB, true>(c, pl, p, batch);
     }
-    static const hipError_t attr0 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, false, KT>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)(WM == 2 ? LDS_BUDGET_MID : LDS_BUDGET));
-    static const hipError_t attr1 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, true, KT>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)(WM == 2 ? LDS_BUDGET_MID : LDS_BUDGET));
+    constexpr int budget = (int)(WM == 2 ? LDS_BUDGET_MID : LDS_BUDGET);
+    static const hipError_t attr0 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, EP_NONE, KT>,
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, budget);
+    static const hipError_t attr1 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, EP_BIAS, KT>,
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, budget);
     FX_HIP_CHECK(attr0);
     FX_HIP_CHECK(attr1);
-    if (p.bias) FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, true, KT>);
-    else FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, false, KT>);
+    if (p.ex.any()) {
+        static const hipError_t attr2 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, EP_FULL, KT>,
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, budget);
+        FX_HIP_CHECK(attr2);
+        FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, EP_FULL, KT>);
+    } else if (p.bias) FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, EP_BIAS, KT>);
+    else FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, EP_NONE, KT>);
     FX_LAUNCH_CHECK();
     return FX_OK;
 }
@@ -345,9 +417,11 @@ inline int launch_tn(fx_ctx* c, const Plan& pl, const Params& p, int batch) {
 }
 
 // A, B and C must be 16-byte aligned.  batch > 1: `batch` products in one launch, operand / result k of the batch sa / sb / sc
-// elements after the first (a stride of 0 shares the operand); bias_per_row: the bias is indexed by the row of C.
+// elements after the first (a stride of 0 shares the operand); bias_per_row: the bias is indexed by the row of C.  ex: one product
+// without bias / relu of its own, the epilogue ex in its store.
 inline int run(fx_ctx* c, const Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K, const float* A, const float* B, float* C,
-               const float* bias, int relu, i64 batch = 1, i64 sa = 0, i64 sb = 0, i64 sc = 0, int bias_per_row = 0) {
+               const float* bias, int relu, i64 batch = 1, i64 sa = 0, i64 sb = 0, i64 sc = 0, int bias_per_row = 0,
+               const gep::Epilogue<float>& ex = gep::Epilogue<float>()) {
     Params p;
     p.A = A; p.B = B; p.C = C; p.bias = bias; p.relu = relu;
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
@@ -357,6 +431,7 @@ inline int run(fx_ctx* c, const Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K,
     p.tiles = pl.tiles_m * pl.tiles_n;
     p.xcd_chunk = p.tiles % 8 == 0 ? p.tiles / 8 : 0;
     p.sa = sa; p.sb = sb; p.sc = sc; p.bias_per_row = bias_per_row;
+    p.ex = ex;
     if (!ta && !tb) return launch_tn<false, false>(c, pl, p, (int)batch);
     if (!ta && tb) return launch_tn<false, true>(c, pl, p, (int)batch);
     if (ta && !tb) return launch_tn<true, false>(c, pl, p, (int)batch);

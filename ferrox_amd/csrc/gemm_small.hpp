@@ -15,7 +15,7 @@
 #pragma once
 #include <cstdlib>
 
-#include "igemm_core.hpp"
+#include "gemm_epilogue.hpp"
 
 namespace gsmall {
 using igemm::f32x16;
@@ -34,6 +34,7 @@ struct Params {
     i64 zstride; // elements between the partial results of consecutive z (0 when K is not split)
     float* asum; // optional (K not split): asum[m] = sum over k of op(A)[m][k], written by the first block of every tile row
     const float* mask;  // optional, [M][N] like C (K not split, no bias): C = (op(A) . op(B)) * (mask > 0 ? 1 : 0), fx_relu_bwd's operation
+    gep::Epilogue<float> ex;  // the EX kernels (K not split): the whole epilogue in place of bias and relu
 };
 
 // KC: 1 = the operand is stored [rows][K] (k contiguous, K % 4 == 0, 16-byte aligned); 2 = the same layout read element by element
@@ -54,7 +55,7 @@ __device__ __forceinline__ void load_group(const float* __restrict__ base, int r
 }
 
 // The work of one block: tile (bx, by) of the product, range bz of K.  red: WAVES * 16 * 64 floats of LDS, rsum: WAVES * 64.
-template <int AKC, int BKC>
+template <int AKC, int BKC, bool EX = false>
 __device__ __forceinline__ void small_body(const Params& p, float* red, float* rsum, int bx, int by, int bz) {
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -62,7 +63,16 @@ __device__ __forceinline__ void small_body(const Params& p, float* red, float* r
     const int am = min(m0 + l32, p.M - 1), bn = min(n0 + l32, p.N - 1);  // past the edge: a valid row / column, result unused
     const int kbase = bz * p.kz, kend = min(p.K, kbase + p.kz);            // this block's range of K (all of it unless K is split over z)
     const int g0 = wave * p.G;
-    const float bias_n = p.bias ? p.bias[bn] : 0.f;  // loaded up front: its latency stays off the closing sum
+    const float* const bias = EX ? p.ex.bias : p.bias;
+    const float bias_n = bias ? bias[bn] : 0.f;  // loaded up front: its latency stays off the closing sum
+    float rs[2] = {0.f, 0.f};                    // likewise the residual's elements
+    if (EX && p.ex.residual) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int e = 2 * wave + u, m = min(m0 + 8 * (e >> 2) + 4 * h + (e & 3), p.M - 1);
+            rs[u] = p.ex.residual[(i64)m * p.N + bn];
+        }
+    }
     float mk[2] = {1.f, 1.f};                        // likewise the mask values of the two elements this lane stores
     if (p.mask) {
 #pragma unroll
@@ -122,7 +132,9 @@ __device__ __forceinline__ void small_body(const Params& p, float* red, float* r
         for (int q = 1; q < WAVES; ++q) v = v + red[(q * 16 + e) * 64 + lane];
         const int m = m0 + 8 * (e >> 2) + 4 * h + (e & 3);
         if (m < p.M && n < p.N) {
-            if (p.bias) {
+            if constexpr (EX) {
+                v = p.ex.finish(v, (i64)m * p.N + n, bias_n, rs[u]);
+            } else if (p.bias) {
                 v = v + bias_n;
                 if (p.relu) v = v > 0.f ? v : 0.f;
             }
@@ -132,11 +144,11 @@ __device__ __forceinline__ void small_body(const Params& p, float* red, float* r
     }
 }
 
-template <int AKC, int BKC>
+template <int AKC, int BKC, bool EX = false>
 __global__ __launch_bounds__(NT) void small_kernel(const Params p) {
     __shared__ float red[WAVES * 16 * 64];
     __shared__ float rsum[WAVES * 64];
-    small_body<AKC, BKC>(p, red, rsum, blockIdx.x, blockIdx.y, blockIdx.z);
+    small_body<AKC, BKC, EX>(p, red, rsum, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // Two independent products in one launch, blockIdx.z picks the product (neither splits K): the data and the weight gradient of a
@@ -163,7 +175,7 @@ __global__ __launch_bounds__(NT) void small_pair_kernel(const Params p0, const P
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int MAXG16 = 16;  // groups of 16 k per wave: K <= 16 * 8 * 16
 
-template <int AKC, int BKC>
+template <int AKC, int BKC, bool EX = false>
 __global__ __launch_bounds__(NT) void small16_kernel(const Params p) {
     __shared__ float red[WAVES * 4 * 64];
     const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, i = lane & 15;
@@ -171,7 +183,10 @@ __global__ __launch_bounds__(NT) void small16_kernel(const Params p) {
     const int m0 = blockIdx.y * 16, n0 = blockIdx.x * 16;
     const int am = min(m0 + i, p.M - 1), bn = min(n0 + i, p.N - 1);  // past the edge: a valid row / column, result unused
     const int g0 = wave * p.G;
-    const float bias_n = p.bias ? p.bias[bn] : 0.f;
+    const float* const bias = EX ? p.ex.bias : p.bias;
+    const float bias_n = bias ? bias[bn] : 0.f;
+    float rs = 0.f;  // the residual's element of the closing sum, loaded up front
+    if (EX && p.ex.residual && wave < 4) rs = p.ex.residual[(i64)min(m0 + 4 * q + wave, p.M - 1) * p.N + bn];
 
     float a[MAXG16][4], b[MAXG16][4];
 #pragma unroll
@@ -205,7 +220,9 @@ __global__ __launch_bounds__(NT) void small16_kernel(const Params p) {
         for (int w = 1; w < WAVES; ++w) v = v + red[(w * 4 + e) * 64 + lane];
         const int m = m0 + 4 * q + e, n = n0 + i;
         if (m < p.M && n < p.N) {
-            if (p.bias) {
+            if constexpr (EX) {
+                v = p.ex.finish(v, (i64)m * p.N + n, bias_n, rs);
+            } else if (p.bias) {
                 v = v + bias_n;
                 if (p.relu) v = v > 0.f ? v : 0.f;
             }
@@ -234,6 +251,7 @@ struct ParamsD {
     i64 zstride;
     double* asum;        // optional, as in Params
     const double* mask;  // optional, as in Params
+    gep::Epilogue<double> ex;  // as in Params
 };
 
 template <int KC>
@@ -252,7 +270,7 @@ __device__ __forceinline__ void load_group_d(const double* __restrict__ base, in
 }
 
 // red_d: [8 waves][16 elements][64 lanes] doubles of LDS
-template <int AKC, int BKC>
+template <int AKC, int BKC, bool EX = false>
 __device__ __forceinline__ void small_body_f64(const ParamsD& p, double* red_d, int bx, int by, int bz) {
     const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -262,7 +280,17 @@ __device__ __forceinline__ void small_body_f64(const ParamsD& p, double* red_d, 
     const int kbase = bz * p.kz, kend = min(p.K, kbase + p.kz);
     const int g0 = wave * p.G;
     // this wave finishes the column block (wave / 2) % 2 in the closing sum; its bias is loaded up front
-    const double bias_n = p.bias ? p.bias[(wave >> 1) & 1 ? bn1 : bn0] : 0.;
+    const double* const bias = EX ? p.ex.bias : p.bias;
+    const double bias_n = bias ? bias[(wave >> 1) & 1 ? bn1 : bn0] : 0.;
+    double rs[2] = {0., 0.};  // the residual's elements of the closing sum
+    if (EX && p.ex.residual) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int el = 2 * wave + u, blk = el >> 2, e = el & 3;
+            const int m = min(m0 + 16 * (blk >> 1) + 4 * e + q, p.M - 1);
+            rs[u] = p.ex.residual[(i64)m * p.N + ((blk & 1) ? bn1 : bn0)];
+        }
+    }
     double mk[2] = {1., 1.};  // the mask values of the two elements this lane stores
     if (p.mask) {
 #pragma unroll
@@ -327,7 +355,9 @@ __device__ __forceinline__ void small_body_f64(const ParamsD& p, double* red_d, 
         for (int w = 1; w < WAVES; ++w) v = v + red_d[(w * 16 + el) * 64 + lane];
         const int m = m0 + 16 * (blk >> 1) + 4 * e + q, n = n0 + 16 * (blk & 1) + l16;
         if (m < p.M && n < p.N) {
-            if (p.bias) {
+            if constexpr (EX) {
+                v = p.ex.finish(v, (i64)m * p.N + n, bias_n, rs[u]);
+            } else if (p.bias) {
                 v = v + bias_n;
                 if (p.relu) v = v > 0. ? v : 0.;
             }
@@ -355,10 +385,10 @@ __device__ __forceinline__ void small_body_f64(const ParamsD& p, double* red_d, 
     }
 }
 
-template <int AKC, int BKC>
+template <int AKC, int BKC, bool EX = false>
 __global__ __launch_bounds__(NT) void small_kernel_f64(const ParamsD p) {
     FX_DYNAMIC_SMEM(double, red_d);
-    small_body_f64<AKC, BKC>(p, red_d, blockIdx.x, blockIdx.y, blockIdx.z);
+    small_body_f64<AKC, BKC, EX>(p, red_d, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 template <int A0>
@@ -425,45 +455,58 @@ template <typename T> inline i64 workspace_bytes(const Plan& pl, i64 M, i64 N) {
 
 // part: workspace_bytes() of scratch when pl.splits > 1 (the caller then adds the partial results, with the bias)
 // asum (optional, only with pl.splits == 1): receives the row sums of op(A)
+// ex: the whole epilogue in place of bias and relu; with K split it rides in the ordered sum, like them
+template <bool EX> inline void launch_f64(fx_ctx* c, const Plan& pl, bool ta, bool tb, dim3 grid, size_t lds, const ParamsD& p) {
+    if (!ta && pl.a_elems && !tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<2, 0, EX>);
+    else if (!ta && pl.a_elems) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<2, 1, EX>);
+    else if (!ta && !tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<1, 0, EX>);
+    else if (!ta && tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<1, 1, EX>);
+    else if (ta && !tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<0, 0, EX>);
+    else FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<0, 1, EX>);
+}
 inline int run_f64(fx_ctx* c, const Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K, const double* A, const double* B, double* C, const double* bias,
-                   int relu, double* part, double* asum = nullptr) {
+                   int relu, double* part, double* asum = nullptr, const gep::Epilogue<double>& ex = gep::Epilogue<double>()) {
     const bool split = pl.splits > 1;
     FX_REQUIRE(!(split && asum), "small product: row sums need an unsplit reduction");
-    ParamsD p{A, B, split ? part : C, split ? nullptr : bias, relu, (int)M, (int)N, (int)K, pl.G, pl.kz, split ? M * N : 0, asum, nullptr};
+    ParamsD p{A, B, split ? part : C, split ? nullptr : bias, relu, (int)M, (int)N, (int)K, pl.G, pl.kz, split ? M * N : 0, asum, nullptr, ex};
     const dim3 grid((unsigned)fx::ceil_div(N, (i64)32), (unsigned)fx::ceil_div(M, (i64)32), (unsigned)pl.splits);
     const size_t lds = (size_t)WAVES * 16 * 64 * sizeof(double);
-    if (!ta && pl.a_elems && !tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<2, 0>);
-    else if (!ta && pl.a_elems) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<2, 1>);
-    else if (!ta && !tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<1, 0>);
-    else if (!ta && tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<1, 1>);
-    else if (ta && !tb) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<0, 0>);
-    else FX_LAUNCH(grid, dim3(NT), lds, c->stream, (p), small_kernel_f64<0, 1>);
+    if (ex.any() && !split) launch_f64<true>(c, pl, ta, tb, grid, lds, p);
+    else launch_f64<false>(c, pl, ta, tb, grid, lds, p);
     FX_LAUNCH_CHECK();
     return FX_OK;
 }
 
+template <bool EX> inline void launch_f32(fx_ctx* c, const Plan& pl, bool ta, bool tb, dim3 grid, const Params& p) {
+    if (!ta && pl.a_elems && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<2, 0, EX>);
+    else if (!ta && pl.a_elems) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<2, 1, EX>);
+    else if (!ta && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<1, 0, EX>);
+    else if (!ta && tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<1, 1, EX>);
+    else if (ta && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<0, 0, EX>);
+    else FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<0, 1, EX>);
+}
+template <bool EX> inline void launch16(fx_ctx* c, bool ta, bool tb, dim3 grid, const Params& p) {
+    if (!ta && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small16_kernel<1, 0, EX>);
+    else if (!ta && tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small16_kernel<1, 1, EX>);
+    else if (ta && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small16_kernel<0, 0, EX>);
+    else FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small16_kernel<0, 1, EX>);
+}
 inline int run(fx_ctx* c, const Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K, const float* A, const float* B, float* C, const float* bias, int relu,
-               float* part, float* asum = nullptr) {
+               float* part, float* asum = nullptr, const gep::Epilogue<float>& ex = gep::Epilogue<float>()) {
     const bool split = pl.splits > 1;
     FX_REQUIRE(!(split && asum), "small product: row sums need an unsplit reduction");
-    Params p{A, B, split ? part : C, split ? nullptr : bias, relu, (int)M, (int)N, (int)K, pl.G, pl.kz, split ? M * N : 0, asum, nullptr};
+    Params p{A, B, split ? part : C, split ? nullptr : bias, relu, (int)M, (int)N, (int)K, pl.G, pl.kz, split ? M * N : 0, asum, nullptr, ex};
     if (pl.tile16) {
         FX_REQUIRE(!split && !asum && !pl.a_elems, "small product: 16 x 16 tiles take neither a split K nor row sums");
         const dim3 grid16((unsigned)fx::ceil_div(N, (i64)16), (unsigned)fx::ceil_div(M, (i64)16));
-        if (!ta && !tb) FX_LAUNCH(grid16, dim3(NT), 0, c->stream, (p), small16_kernel<1, 0>);
-        else if (!ta && tb) FX_LAUNCH(grid16, dim3(NT), 0, c->stream, (p), small16_kernel<1, 1>);
-        else if (ta && !tb) FX_LAUNCH(grid16, dim3(NT), 0, c->stream, (p), small16_kernel<0, 0>);
-        else FX_LAUNCH(grid16, dim3(NT), 0, c->stream, (p), small16_kernel<0, 1>);
+        if (ex.any()) launch16<true>(c, ta, tb, grid16, p);
+        else launch16<false>(c, ta, tb, grid16, p);
         FX_LAUNCH_CHECK();
         return FX_OK;
     }
     const dim3 grid((unsigned)fx::ceil_div(N, (i64)32), (unsigned)fx::ceil_div(M, (i64)32), (unsigned)pl.splits);
-    if (!ta && pl.a_elems && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<2, 0>);
-    else if (!ta && pl.a_elems) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<2, 1>);
-    else if (!ta && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<1, 0>);
-    else if (!ta && tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<1, 1>);
-    else if (ta && !tb) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<0, 0>);
-    else FX_LAUNCH(grid, dim3(NT), 0, c->stream, (p), small_kernel<0, 1>);
+    if (ex.any() && !split) launch_f32<true>(c, pl, ta, tb, grid, p);
+    else launch_f32<false>(c, pl, ta, tb, grid, p);
     FX_LAUNCH_CHECK();
     return FX_OK;
 }
@@ -474,8 +517,8 @@ inline int run(fx_ctx* c, const Plan& pl, bool ta, bool tb, i64 M, i64 N, i64 K,
 inline int run_pair(fx_ctx* c, const Plan& p0, const Plan& p1, i64 M0, i64 N0, i64 K0, const float* A0, const float* B0, float* C0, i64 M1, i64 N1,
                     i64 K1, const float* A1, const float* B1, float* C1, float* asum1, const float* mask0) {
     FX_REQUIRE(p0.splits == 1 && p1.splits == 1, "small product pair: unsplit reductions only");
-    Params a{A0, B0, C0, nullptr, 0, (int)M0, (int)N0, (int)K0, p0.G, p0.kz, 0, nullptr, mask0};
-    Params b{A1, B1, C1, nullptr, 0, (int)M1, (int)N1, (int)K1, p1.G, p1.kz, 0, asum1, nullptr};
+    Params a{A0, B0, C0, nullptr, 0, (int)M0, (int)N0, (int)K0, p0.G, p0.kz, 0, nullptr, mask0, {}};
+    Params b{A1, B1, C1, nullptr, 0, (int)M1, (int)N1, (int)K1, p1.G, p1.kz, 0, asum1, nullptr, {}};
     const dim3 grid((unsigned)fx::ceil_div(std::max(N0, N1), (i64)32), (unsigned)fx::ceil_div(std::max(M0, M1), (i64)32), 2);
     if (p0.a_elems) FX_LAUNCH(grid, dim3(NT), 0, c->stream, (a, b), small_pair_kernel<2>);
     else FX_LAUNCH(grid, dim3(NT), 0, c->stream, (a, b), small_pair_kernel<1>);
@@ -485,8 +528,8 @@ inline int run_pair(fx_ctx* c, const Plan& p0, const Plan& p1, i64 M0, i64 N0, i
 inline int run_pair(fx_ctx* c, const Plan& p0, const Plan& p1, i64 M0, i64 N0, i64 K0, const double* A0, const double* B0, double* C0, i64 M1,
                     i64 N1, i64 K1, const double* A1, const double* B1, double* C1, double* asum1, const double* mask0) {
     FX_REQUIRE(p0.splits == 1 && p1.splits == 1, "small product pair: unsplit reductions only");
-    ParamsD a{A0, B0, C0, nullptr, 0, (int)M0, (int)N0, (int)K0, p0.G, p0.kz, 0, nullptr, mask0};
-    ParamsD b{A1, B1, C1, nullptr, 0, (int)M1, (int)N1, (int)K1, p1.G, p1.kz, 0, asum1, nullptr};
+    ParamsD a{A0, B0, C0, nullptr, 0, (int)M0, (int)N0, (int)K0, p0.G, p0.kz, 0, nullptr, mask0, {}};
+    ParamsD b{A1, B1, C1, nullptr, 0, (int)M1, (int)N1, (int)K1, p1.G, p1.kz, 0, asum1, nullptr, {}};
     const dim3 grid((unsigned)fx::ceil_div(std::max(N0, N1), (i64)32), (unsigned)fx::ceil_div(std::max(M0, M1), (i64)32), 2);
     const size_t lds = (size_t)WAVES * 16 * 64 * sizeof(double);
     if (p0.a_elems) FX_LAUNCH(grid, dim3(NT), lds, c->stream, (a, b), small_pair_kernel_f64<2>);

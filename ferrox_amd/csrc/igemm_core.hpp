@@ -603,9 +603,8 @@ template <typename T> struct SumEpilogue {
     }
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void splitk_reduce_kernel(const T* __restrict__ part, T* __restrict__ out, i64 n, int splits,
-                                                            const SumEpilogue<T> ep = SumEpilogue<T>()) {
+template <typename T, class SE = SumEpilogue<T>>
+__global__ __launch_bounds__(256) void splitk_reduce_kernel(const T* __restrict__ part, T* __restrict__ out, i64 n, int splits, const SE ep = SE()) {
     const i64 i = (i64)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     T s = T(0);
@@ -649,9 +648,8 @@ int launch_multi(fx_ctx* c, const MultiProblem<AL, BL, EP, NP>& mp, int count) {
 // Same sum for few outputs and many splits: G threads share one output, thread g adds splits g, g+G, ... in
 // order, then the G partial sums are added in order of g.  The grouping depends only on (n, splits), so the
 // result is reproducible run to run; it differs from the single-chain order by rounding only.
-template <typename T, int G>
-__global__ __launch_bounds__(256) void splitk_reduce_grouped_kernel(const T* __restrict__ part, T* __restrict__ out, i64 n, int splits,
-                                                                    const SumEpilogue<T> ep = SumEpilogue<T>()) {
+template <typename T, int G, class SE = SumEpilogue<T>>
+__global__ __launch_bounds__(256) void splitk_reduce_grouped_kernel(const T* __restrict__ part, T* __restrict__ out, i64 n, int splits, const SE ep = SE()) {
     constexpr int COLS = 256 / G;
     __shared__ T sm[G][COLS];
     const int col = threadIdx.x % COLS, g = threadIdx.x / COLS;
@@ -678,6 +676,17 @@ __global__ __launch_bounds__(256) void splitk_reduce_grouped_kernel(const T* __r
     }
 }
 
+template <typename T, class SE>
+int launch_splitk_reduce_with(fx_ctx* c, const T* part, T* out, i64 n, int splits, const SE& ep) {
+    if (splits >= 128 && n <= (1 << 16))
+        FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 16)), dim3(256), 0, c->stream, (part, out, n, splits, ep), splitk_reduce_grouped_kernel<T, 16, SE>);
+    else if (splits >= 32 && n <= (1 << 18))
+        FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 64)), dim3(256), 0, c->stream, (part, out, n, splits, ep), splitk_reduce_grouped_kernel<T, 4, SE>);
+    else
+        FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 256)), dim3(256), 0, c->stream, (part, out, n, splits, ep), splitk_reduce_kernel<T, SE>);
+    FX_LAUNCH_CHECK();
+    return FX_OK;
+}
 // bias (with ncols, relu): the epilogue above; n must then fit 32 bits
 template <typename T>
 int launch_splitk_reduce(fx_ctx* c, const T* part, T* out, i64 n, int splits, const T* bias = nullptr, i64 ncols = 1, int relu = 0) {
@@ -686,14 +695,7 @@ int launch_splitk_reduce(fx_ctx* c, const T* part, T* out, i64 n, int splits, co
         FX_REQUIRE(n <= 0x7fffffff && ncols >= 1 && ncols <= 0x7fffffff, "split-K sum with bias: %lld outputs exceed 2^31", (long long)n);
         ep.bias = bias; ep.ncols = (int)ncols; ep.relu = relu; ep.div_cols = FastDiv((uint32_t)ncols);
     }
-    if (splits >= 128 && n <= (1 << 16))
-        FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 16)), dim3(256), 0, c->stream, (part, out, n, splits, ep), splitk_reduce_grouped_kernel<T, 16>);
-    else if (splits >= 32 && n <= (1 << 18))
-        FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 64)), dim3(256), 0, c->stream, (part, out, n, splits, ep), splitk_reduce_grouped_kernel<T, 4>);
-    else
-        FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 256)), dim3(256), 0, c->stream, (part, out, n, splits, ep), splitk_reduce_kernel<T>);
-    FX_LAUNCH_CHECK();
-    return FX_OK;
+    return launch_splitk_reduce_with<T>(c, part, out, n, splits, ep);
 }
 
 // Partial sums that carry a second, short result behind the first ([n1] then [n2] floats per split, `stride` apart): both are
