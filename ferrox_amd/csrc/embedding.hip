@@ -121,82 +121,13 @@ __device__ __forceinline__ void scan_counts(uint32_t* counts, uint32_t* wsum) {
     __syncthreads();
 }
 
-// The one-launch sort: block b owns ids 256 b .. 256 b + 255 (the last block also the padding key `vocab`), n <= 1024 K.
-// Reading: thread t of wave w holds tokens (w K + j) 64 + lane, all loads in flight at once.
-template <int K>
-__global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __restrict__ ids, uint32_t* __restrict__ keys, uint32_t* __restrict__ pos,
-                                                             int n, i64 vocab) {
-    FX_DYNAMIC_SMEM(uint32_t, smem);
-    uint32_t* counts = smem;                                   // [SORT_WAVES][BINS]
-    uint32_t* start = counts + SORT_WAVES * BINS;              // [BINS]: where the next item of a digit goes
-    uint32_t* wsum = start + BINS;                             // 4
-    uint32_t* inside = wsum + 4;                               // [SORT_WAVES]: tokens of this block's ids per wave
-    uint32_t* below = inside + SORT_WAVES;                     // [SORT_WAVES]: tokens of smaller ids per wave
-    uint16_t* lpos = reinterpret_cast<uint16_t*>(below + SORT_WAVES);  // [K * SORT_NT]: the kept tokens, in order
-    uint8_t* ldig = reinterpret_cast<uint8_t*>(lpos + K * SORT_NT);
-    constexpr int R = K < 4 ? K : 4;  // kept tokens per thread and round
+// The kept tokens of the one-launch sort to their places: rounds of R tokens per thread.  m tokens with digits ldig and positions lpos,
+// in order; start [BINS] (more than one round): where the next item of a digit goes; one round: its own scan and base say it.
+template <int R>
+__device__ __forceinline__ void place_items(uint32_t* __restrict__ keys, uint32_t* __restrict__ pos, uint32_t lo, uint32_t base, uint32_t m,
+                                            const uint16_t* lpos, const uint8_t* ldig, uint32_t* counts, uint32_t* start, uint32_t* wsum) {
     constexpr uint32_t ROUND = R * SORT_NT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t lo = blockIdx.x * BINS;
-    uint32_t key[K];
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-        const int i = (wave * K + j) * 64 + lane;
-        key[j] = i < n ? key_of(ids[i], vocab) : 0xffffffffu;
-    }
-    uint32_t in = 0, lt = 0;
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-        in += (uint32_t)__popcll(__ballot(key[j] - lo < (uint32_t)BINS));
-        lt += (uint32_t)__popcll(__ballot(key[j] < lo));
-    }
-    if (lane == 0) {
-        inside[wave] = in;
-        below[wave] = lt;
-    }
-    if (threadIdx.x < BINS) start[threadIdx.x] = 0;
-    __syncthreads();
-    uint32_t at = 0, m = 0, base = 0;
-#pragma unroll
-    for (int w = 0; w < SORT_WAVES; ++w) {
-        if (w < wave) at += inside[w];
-        m += inside[w];
-        base += below[w];
-    }
-    if (m == 0) return;  // block-uniform
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-        const uint32_t d = key[j] - lo;
-        const bool mine = d < (uint32_t)BINS;
-        const uint64_t who = __ballot(mine);
-        if (mine) {
-            const uint32_t to = at + (uint32_t)__popcll(who & ((1ull << lane) - 1));
-            lpos[to] = (uint16_t)((wave * K + j) * 64 + lane);
-            ldig[to] = (uint8_t)d;
-            if (m > ROUND) atomicAdd(&start[d], 1u);  // whole numbers: any order
-        }
-        at += (uint32_t)__popcll(who);
-    }
-    __syncthreads();
-    // where each digit begins: with one round its own scan says it, with more of them the digits were counted above
-    if (m > ROUND) {  // block-uniform
-        uint32_t sum = 0, incl = 0;
-        if (threadIdx.x < BINS) {
-            sum = incl = start[threadIdx.x];
-#pragma unroll
-            for (int q = 1; q < 64; q <<= 1) {
-                const uint32_t o = __shfl_up(incl, q, 64);
-                if (lane >= q) incl += o;
-            }
-            if (lane == 63) wsum[wave] = incl;
-        }
-        __syncthreads();
-        if (threadIdx.x < BINS) {
-            uint32_t s = base + incl - sum;
-            for (int w = 0; w < wave; ++w) s += wsum[w];
-            start[threadIdx.x] = s;
-        }
-    }
     for (uint32_t r = 0; r < m; r += ROUND) {
         uint32_t dig[R], rank[R];
 #pragma unroll
@@ -227,24 +158,103 @@ __global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __re
     }
 }
 
+// The one-launch sort: block b owns ids 256 b .. 256 b + 255 (the last block also the padding key `vocab`), n <= 1024 K.
+// Reading: thread t of wave w holds tokens (w K + j) 64 + lane, all loads in flight at once.  Every block looks at every token, so
+// what is done per token is kept to two comparisons and counts per lane; the few tokens of the block's own ids are then placed.
+template <int K>
+__global__ __launch_bounds__(SORT_NT) void sort_range_kernel(const int64_t* __restrict__ ids, uint32_t* __restrict__ keys, uint32_t* __restrict__ pos,
+                                                             int n, i64 vocab) {
+    FX_DYNAMIC_SMEM(uint32_t, smem);
+    uint32_t* counts = smem;                                   // [SORT_WAVES][BINS]
+    uint32_t* start = counts + SORT_WAVES * BINS;              // [BINS]
+    uint32_t* wsum = start + BINS;                             // 4
+    uint32_t* inside = wsum + 4;                               // [SORT_WAVES]: tokens of this block's ids per wave
+    uint32_t* below = inside + SORT_WAVES;                     // [SORT_WAVES]: tokens of smaller ids per wave
+    uint16_t* lpos = reinterpret_cast<uint16_t*>(below + SORT_WAVES);  // [K * SORT_NT]: the kept tokens, in order
+    uint8_t* ldig = reinterpret_cast<uint8_t*>(lpos + K * SORT_NT);
+    constexpr int RL = K < 4 ? K : 4;                          // tokens per thread and round of a long list
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t lo = blockIdx.x * BINS;
+    uint32_t key[K];
+    {
+        int64_t id[K];  // unconditional loads: a branch around each would make them wait for one another
+#pragma unroll
+        for (int j = 0; j < K; ++j) id[j] = ids[min((wave * K + j) * 64 + lane, n - 1)];
+#pragma unroll
+        for (int j = 0; j < K; ++j) key[j] = (wave * K + j) * 64 + lane < n ? key_of(id[j], vocab) : 0xffffffffu;
+    }
+    uint32_t both = 0;  // tokens of this block's ids in the low half, of smaller ids in the high half: at most 64 K = 2048 per wave
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const uint32_t d = key[j] - lo;
+        both += d < (uint32_t)BINS ? 1u : 0u;
+        both += key[j] < lo ? 0x10000u : 0u;
+    }
+    both = wave_sum(both);
+    if (lane == 0) {
+        inside[wave] = both & 0xffffu;
+        below[wave] = both >> 16;
+    }
+    if (threadIdx.x < BINS) start[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t at = 0, m = 0, base = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+        if (w < wave) at += inside[w];
+        m += inside[w];
+        base += below[w];
+    }
+    if (m == 0) return;  // block-uniform
+    const bool many = m > RL * SORT_NT;  // more than one round: the digits are counted beforehand
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const uint32_t d = key[j] - lo;
+        const bool mine = d < (uint32_t)BINS;
+        const uint64_t who = __ballot(mine);
+        if (who) {  // wave-uniform
+            if (mine) {
+                const uint32_t to = at + (uint32_t)__popcll(who & ((1ull << lane) - 1));
+                lpos[to] = (uint16_t)((wave * K + j) * 64 + lane);
+                ldig[to] = (uint8_t)d;
+                if (many) atomicAdd(&start[d], 1u);  // whole numbers: any order
+            }
+            at += (uint32_t)__popcll(who);
+        }
+    }
+    __syncthreads();
+    if (many) {  // block-uniform
+        uint32_t sum = 0, incl = 0;
+        if (threadIdx.x < BINS) {
+            sum = incl = start[threadIdx.x];
+#pragma unroll
+            for (int q = 1; q < 64; q <<= 1) {
+                const uint32_t o = __shfl_up(incl, q, 64);
+                if (lane >= q) incl += o;
+            }
+            if (lane == 63) wsum[wave] = incl;
+        }
+        __syncthreads();
+        if (threadIdx.x < BINS) {
+            uint32_t s = base + incl - sum;
+            for (int w = 0; w < wave; ++w) s += wsum[w];
+            start[threadIdx.x] = s;
+        }
+    }
+    if (m <= SORT_NT) place_items<1>(keys, pos, lo, base, m, lpos, ldig, counts, start, wsum);
+    else place_items<RL>(keys, pos, lo, base, m, lpos, ldig, counts, start, wsum);
+}
+
 // One radix pass over many tiles.  The first pass reads the ids themselves (keys_in == null).
 constexpr int TILE_K = TILE / SORT_NT;
 __device__ __forceinline__ void tile_items(const int64_t* ids, const uint32_t* keys_in, const uint32_t* pos_in, i64 n, i64 vocab, uint32_t (&key)[TILE_K],
                                            uint32_t (&at)[TILE_K]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int j = 0; j < TILE_K; ++j) {
-        const i64 i = (i64)blockIdx.x * TILE + (wave * TILE_K + j) * 64 + lane;
-        key[j] = 0xffffffffu;
-        at[j] = (uint32_t)i;
-        if (i < n) {
-            if (keys_in) {
-                key[j] = keys_in[i];
-                at[j] = pos_in[i];
-            } else {
-                key[j] = key_of(ids[i], vocab);
-            }
-        }
+    for (int j = 0; j < TILE_K; ++j) {  // unconditional loads (the last token again past the end), all in flight
+        const i64 i = (i64)blockIdx.x * TILE + (wave * TILE_K + j) * 64 + lane, ic = min(i, n - 1);
+        key[j] = keys_in ? keys_in[ic] : key_of(ids[ic], vocab);
+        at[j] = keys_in ? pos_in[ic] : (uint32_t)i;
+        if (i >= n) key[j] = 0xffffffffu;
     }
 }
 __global__ __launch_bounds__(SORT_NT) void sort_count_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys_in, i64 n, i64 vocab,
@@ -252,10 +262,15 @@ __global__ __launch_bounds__(SORT_NT) void sort_count_kernel(const int64_t* __re
     __shared__ uint32_t hist[BINS];
     for (int b = threadIdx.x; b < BINS; b += SORT_NT) hist[b] = 0;
     __syncthreads();
+    uint32_t key[TILE_K];
+#pragma unroll
     for (int j = 0; j < TILE_K; ++j) {
-        const i64 i = (i64)blockIdx.x * TILE + j * SORT_NT + threadIdx.x;
-        if (i < n) atomicAdd(&hist[((keys_in ? keys_in[i] : key_of(ids[i], vocab)) >> shift) & (BINS - 1)], 1u);  // whole numbers: any order
+        const i64 i = min((i64)blockIdx.x * TILE + j * SORT_NT + threadIdx.x, n - 1);
+        key[j] = keys_in ? keys_in[i] : key_of(ids[i], vocab);
     }
+#pragma unroll
+    for (int j = 0; j < TILE_K; ++j)
+        if ((i64)blockIdx.x * TILE + j * SORT_NT + threadIdx.x < n) atomicAdd(&hist[(key[j] >> shift) & (BINS - 1)], 1u);  // whole numbers: any order
     __syncthreads();
     for (int b = threadIdx.x; b < BINS; b += SORT_NT) table[(i64)b * tiles + blockIdx.x] = hist[b];
 }
