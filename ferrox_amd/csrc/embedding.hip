@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void embedding_add_kernel(const T* __restrict_
         const int nv = (int)((c1 - c0) / V);
         for (int i = threadIdx.x; i < ZROWS * nv; i += 256) {
             const int r = i / nv;
-            if (!present[r]) store<V>(dW + (v0 + r) * a.D + c0 + (i64)(i - r * nv) * V, zero);
+            if (!present[r]) store_stream<V>(dW + (v0 + r) * a.D + c0 + (i64)(i - r * nv) * V, zero);
         }
         return;
     }
@@ -438,11 +438,11 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t* __r
                                                              const Add a) {
     __shared__ T sm[4][64 * V];
     const i64 b = blockIdx.x, border = (b + 1) * a.P;  // < n
-    const uint32_t k = keys[border];
-    if (k >= (uint32_t)a.vocab || keys[border - 1] != k) return;       // block-uniform, as all exits here
-    const i64 first = b * a.P;                                          // piece b's first position
-    const bool whole = keys[first] == k;                                // the run holds all of piece b
-    if (whole && first > 0 && keys[first - 1] == k) return;             // an earlier border has it
+    const i64 first = b * a.P;  // piece b's first position
+    const uint32_t k = keys[border], k1 = keys[border - 1], kf = keys[first], kb = keys[first > 0 ? first - 1 : 0];  // in flight together
+    const bool whole = kf == k;                                // the run holds all of piece b
+    // no run crosses here, or an earlier border has it (block-uniform)
+    if ((k >= (uint32_t)a.vocab) | (k1 != k) | (whole & (first > 0) & (kb == k))) return;
     // the run's last piece: the first from b + 1 on that is the last one or ends before the run does; 64 pieces are looked at together
     const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
     i64 end = b + 1;

@@ -20,6 +20,13 @@ template <int V, typename T> __device__ __forceinline__ void store(T* p, const T
     for (int u = 0; u < V; ++u) q[u] = v[u];
     *reinterpret_cast<Vec<T, V>*>(p) = q;
 }
+// past the caches: large outputs that nothing reads soon
+template <int V, typename T> __device__ __forceinline__ void store_stream(T* p, const T (&v)[V]) {
+    Vec<T, V> q;
+#pragma unroll
+    for (int u = 0; u < V; ++u) q[u] = v[u];
+    __builtin_nontemporal_store(q, reinterpret_cast<Vec<T, V>*>(p));
+}
 
 // The vector at column j of a row that ends at D: whole, or what is left of the row (the rest zero / not stored).
 template <int V, typename T> __device__ __forceinline__ void load_part(const T* row, int j, int D, T (&v)[V]) {
