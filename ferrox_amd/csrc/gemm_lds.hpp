@@ -4,17 +4,17 @@
 //
 // A block (4 waves) owns a BM x BN tile, BM = 32*WM, BN = 32*TN*(4/WM): the waves are laid out WM x (4/WM); a wave owns 32
 // rows and 32*TN columns, i.e. TN accumulator blocks of 32x32 (v_mfma_f32_32x32x2_f32).  Large products take 128 x 128 or
-// 128 x 64 tiles (WM = 4, TN = 4 or 2); products with too few of those to fill the chip (1024^3: 64 tiles) take 64 x 128 or
-// 64 x 64 tiles (WM = 2, TN = 2 or 1) instead of a K split with partial sums in memory; with one accumulator block per wave
-// the even and the odd MFMA steps add into two accumulators (added once at the end), so that no MFMA waits for the one
-// before it.  Per stage (KC = 64 values of k) LDS holds both operand
-// slabs in the form their memory layout gives for free:
+// 128 x 64 tiles (WM = 4, TN = 4 or 2; gemm_pipe_kernel, 32-deep stages); products with too few of those to fill the chip (1024^3:
+// 64 tiles) take 64 x 128 or 64 x 64 tiles (WM = 2, TN = 2 or 1; gemm_lds_kernel, 64-deep stages) instead of a K split with partial
+// sums in memory; with one accumulator block per wave the even and the odd MFMA steps add into two accumulators (added once at the
+// end), so that no MFMA waits for the one before it.
+// In the 64-deep stages LDS holds both operand slabs in the form their memory layout gives for free:
 //   k-contiguous operand (A as stored [M,K]; B given as [N,K]):  S[r][k], pitch 65  -> the 32 lanes of an MFMA operand
 //                                                               read (r = lane % 32, k + lane / 32) hit 32 banks
-//   row-contiguous operand (A given as [K,M]; B as stored [K,N]): S[k][r], pitch 128 / BN -> lanes read 32 consecutive floats
+//   row-contiguous operand (A given as [K,M]; B as stored [K,N]): S[k][r], pitch BM / BN -> lanes read 32 consecutive floats
 // so staging is a straight copy of 16-byte global loads (four 4-byte LDS stores for the odd pitch, one 16-byte store
 // otherwise) and the MFMA loop contains nothing but LDS reads with compile-time offsets.  The next stage's global
-// loads are issued before the MFMA loop of the current stage and parked in registers; two blocks share a CU.
+// loads are issued before the MFMA loop of the current stage and parked in registers.
 // Workgroup ids are handed to the eight XCDs round-robin by the hardware; the id -> tile map gives each XCD a
 // contiguous range of tiles so that the tiles resident on one XCD share operand panels in its L2.
 #pragma once
@@ -26,7 +26,6 @@ using igemm::ldg4;
 
 constexpr int KC = 64, NT = 256;
 constexpr int PK = KC + 1;  // pitch of a k-contiguous slab row
-constexpr size_t LDS_BUDGET = 72 * 1024;       // one stage of the 128-row tiles: two blocks per CU
 constexpr size_t LDS_BUDGET_MID = 104 * 1024;  // two stages of the 64-row tiles (one block per CU has to overlap by itself)
 
 struct Params {
@@ -45,18 +44,105 @@ struct Params {
 };
 constexpr int EP_NONE = 0, EP_BIAS = 1, EP_FULL = 2;  // what the store does: nothing, bias (+ ReLU), the whole of gep::Epilogue
 
+// The store of one wave's 32 x 32 TN block of the tile, rows from m0, columns from n0.  smem: the block's LDS, which nobody reads any more.
+template <int TN, int EP, int NACC>
+__device__ __forceinline__ void store_tile(const Params& p, float* Cb, float* smem, f32x16 (&acc)[NACC], int m0, int n0, int lane, int wave) {
+    const int l32 = lane & 31;
+    if constexpr (EP == EP_FULL) {
+        // Each wave turns its 32 rows through LDS (its own piece; every wave has left the slabs through the barrier that ended the
+        // last stage), 16-byte groups along a row then, so that bias, residual, pre and C move in 16-byte accesses and the
+        // activation is compiled for four elements instead of 16 TN.
+        constexpr int WC = 32 * TN, CG = WC / 4, RPI = 64 / CG;  // columns of the wave, groups per row, rows per pass
+        float* const turn = smem + wave * (32 * WC);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) turn[igemm::Mfma<float>::row(e, lane) * WC + j * 32 + l32] = acc[j][e];
+        __syncthreads();
+        const int n = n0 + 4 * (lane % CG), left = p.N - n;
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.ex.bias) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q < left) bias[q] = p.ex.bias[n + q];
+        }
+#pragma unroll 1
+        for (int r = lane / CG; r < 32; r += RPI) {
+            const int m = m0 + r;
+            if (m >= p.M || left <= 0) continue;
+            const i64 i = (i64)m * p.N + n;
+            const float4 t4 = *reinterpret_cast<const float4*>(turn + r * WC + 4 * (lane % CG));
+            float v[4] = {t4.x, t4.y, t4.z, t4.w}, res[4] = {0.f, 0.f, 0.f, 0.f};
+            typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // a row of C starts at any element
+            if (p.ex.residual) {
+                if (left >= 4) {
+                    const f4u q4 = *reinterpret_cast<const f4u*>(p.ex.residual + i);
+                    res[0] = q4.x; res[1] = q4.y; res[2] = q4.z; res[3] = q4.w;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        if (q < left) res[q] = p.ex.residual[i + q];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (p.ex.bias) v[q] = v[q] + bias[q];
+            if (p.ex.pre) {
+                if (left >= 4) {
+                    *reinterpret_cast<f4u*>(p.ex.pre + i) = f4u{v[0], v[1], v[2], v[3]};
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        if (q < left) p.ex.pre[i + q] = v[q];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[q] = fxact::apply<float>(p.ex.act, v[q]);
+                if (p.ex.residual) v[q] = v[q] + res[q];
+            }
+            if (left >= 4) {
+                *reinterpret_cast<f4u*>(Cb + i) = f4u{v[0], v[1], v[2], v[3]};
+            } else {
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+                    if (q < left) Cb[i + q] = v[q];
+            }
+        }
+        return;
+    }
+    constexpr bool BIAS = EP == EP_BIAS;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int n = n0 + j * 32 + l32;
+        const float bj = BIAS && !p.bias_per_row ? p.bias[n < p.N ? n : p.N - 1] : 0.f;
+        if (n < p.N) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = m0 + igemm::Mfma<float>::row(e, lane);
+                if (m < p.M) {
+                    float v = acc[j][e];
+                    if (BIAS) {
+                        v = v + (p.bias_per_row ? p.bias[m] : bj);
+                        if (p.relu) v = v > 0.f ? v : 0.f;
+                    }
+                    Cb[(i64)m * p.N + n] = v;
+                }
+            }
+        }
+    }
+}
+
 // TA: A is stored [K, M] (m contiguous); TB: B is stored [N, K] (k contiguous).
 // KT (both operands k-contiguous only): K need not be a multiple of the stage depth -- the last stage loads what is left of the rows
 // (K a multiple of 4: a 16-byte vector is inside a row or past it) and parks zeros behind it.
-template <int TN, int WM, bool TA, bool TB, int EP, bool KT = false>
+// The 64-row tiles (WM = 2).  They run where there is about one block per CU, so LDS keeps two stages: the next stage is parked while
+// other waves still compute and a stage costs one barrier.
+template <int TN, bool TA, bool TB, int EP, bool KT = false>
 __global__ __launch_bounds__(NT, 2) void gemm_lds_kernel(const Params p) {
     static_assert(!KT || (!TA && TB), "the K tail is handled for k-contiguous operands");
-    constexpr int WN = 4 / WM, BM = 32 * WM, BN = 32 * TN * WN;
+    constexpr int WM = 2, WN = 4 / WM, BM = 32 * WM, BN = 32 * TN * WN;
     constexpr int NACC = TN == 1 ? 2 : TN;  // accumulator blocks of a wave (TN == 1: even and odd MFMA steps apart)
-    // The 128-row tiles keep one stage in LDS and rely on the CU's second block to cover staging; the 64-row tiles run where
-    // there is about one block per CU, so they keep two stages: the next stage is parked while other waves still compute and a
-    // stage costs one barrier.
-    constexpr int STAGES = WM == 2 ? 2 : 1;
     constexpr int PA = TA ? BM : PK, PB = TB ? PK : BN;          // LDS pitches
     constexpr int ASZ = TA ? KC * BM : BM * PK, BSZ = TB ? BN * PK : KC * BN;
     constexpr int NA = BM * KC / 4 / NT, NB = BN * KC / 4 / NT;  // float4 per thread per stage
@@ -182,43 +268,32 @@ __global__ __launch_bounds__(NT, 2) void gemm_lds_kernel(const Params p) {
             }
             __builtin_amdgcn_sched_barrier(0);
         };
-        if constexpr (STAGES == 2) {
-            // one block per CU, one wave per SIMD: the operand reads run two MFMA steps ahead (three register sets), which
-            // covers the LDS latency that a second wave would otherwise hide
-            float a2, b2[TN];
-            rd(a0, b0, 0);
-            rd(a1, b1, 1);
+        // one block per CU, one wave per SIMD: the operand reads run two MFMA steps ahead (three register sets), which
+        // covers the LDS latency that a second wave would otherwise hide
+        float a2, b2[TN];
+        rd(a0, b0, 0);
+        rd(a1, b1, 1);
 #pragma unroll
-            for (int s = 0; s < KC / 2; s += 6) {
-                if (s + 2 < KC / 2) rd(a2, b2, s + 2);
-                mma(a0, b0, 0);
-                if (s + 3 < KC / 2) rd(a0, b0, s + 3);
-                mma(a1, b1, 1);
-                if (s + 2 < KC / 2) {
-                    if (s + 4 < KC / 2) rd(a1, b1, s + 4);
-                    mma(a2, b2, 0);
-                }
-                if (s + 3 < KC / 2) {
-                    if (s + 5 < KC / 2) rd(a2, b2, s + 5);
-                    mma(a0, b0, 1);
-                }
-                if (s + 4 < KC / 2) {
-                    if (s + 6 < KC / 2) rd(a0, b0, s + 6);
-                    mma(a1, b1, 0);
-                }
-                if (s + 5 < KC / 2) {
-                    if (s + 7 < KC / 2) rd(a1, b1, s + 7);
-                    mma(a2, b2, 1);
-                }
+        for (int s = 0; s < KC / 2; s += 6) {
+            if (s + 2 < KC / 2) rd(a2, b2, s + 2);
+            mma(a0, b0, 0);
+            if (s + 3 < KC / 2) rd(a0, b0, s + 3);
+            mma(a1, b1, 1);
+            if (s + 2 < KC / 2) {
+                if (s + 4 < KC / 2) rd(a1, b1, s + 4);
+                mma(a2, b2, 0);
             }
-        } else {
-            rd(a0, b0, 0);
-#pragma unroll
-            for (int s = 0; s < KC / 2; s += 2) {
-                rd(a1, b1, s + 1);
-                mma(a0, b0, 0);
-                if (s + 2 < KC / 2) rd(a0, b0, s + 2);
-                mma(a1, b1, 1);
+            if (s + 3 < KC / 2) {
+                if (s + 5 < KC / 2) rd(a2, b2, s + 5);
+                mma(a0, b0, 1);
+            }
+            if (s + 4 < KC / 2) {
+                if (s + 6 < KC / 2) rd(a0, b0, s + 6);
+                mma(a1, b1, 0);
+            }
+            if (s + 5 < KC / 2) {
+                if (s + 7 < KC / 2) rd(a1, b1, s + 7);
+                mma(a2, b2, 1);
             }
         }
     };
@@ -226,117 +301,198 @@ __global__ __launch_bounds__(NT, 2) void gemm_lds_kernel(const Params p) {
     prefetch(0);
     park(0);
     __syncthreads();
-    if constexpr (STAGES == 1) {
-        for (int k0 = 0; k0 < p.K; k0 += KC) {
-            const bool more = k0 + KC < p.K;
-            if (more) prefetch(k0 + KC);
-            __builtin_amdgcn_s_setprio(3);  // a co-resident block that is staging must not delay these MFMAs
-            compute(0);
-            __builtin_amdgcn_s_setprio(0);
-            __syncthreads();
-            if (more) park(0);
-            __syncthreads();
-        }
-    } else {
-        int cur = 0;
-        for (int k0 = 0; k0 < p.K; k0 += KC) {
-            const bool more = k0 + KC < p.K;
-            if (more) prefetch(k0 + KC);
-            compute(cur);
-            // the other buffer was last read in the stage before this one, which every wave has left through the barrier below
-            if (more) park(cur ^ 1);
-            __syncthreads();
-            cur ^= 1;
-        }
+    int cur = 0;
+    for (int k0 = 0; k0 < p.K; k0 += KC) {
+        const bool more = k0 + KC < p.K;
+        if (more) prefetch(k0 + KC);
+        compute(cur);
+        // the other buffer was last read in the stage before this one, which every wave has left through the barrier below
+        if (more) park(cur ^ 1);
+        __syncthreads();
+        cur ^= 1;
     }
 
     if constexpr (TN == 1) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[0][e] = acc[0][e] + acc[1][e];
     }
-    if constexpr (EP == EP_FULL) {
-        // Each wave turns its 32 rows through LDS (its own piece; every wave has left the slabs through the barrier that ended the
-        // last stage), 16-byte groups along a row then, so that bias, residual, pre and C move in 16-byte accesses and the
-        // activation is compiled for four elements instead of 16 TN.  Measured at 4096 x 1024 x 4096 with bias and residual: see gemm.hip.
-        constexpr int WC = 32 * TN, CG = WC / 4, RPI = 64 / CG;  // columns of the wave, groups per row, rows per pass
-        float* const turn = smem + wave * (32 * WC);
+    store_tile<TN, EP>(p, Cb, smem, acc, m0 + wm * 32, n0 + wn * 32 * TN, lane, wave);
+}
+
+// The 128-row tiles (WM = 4), with two stages of 32 k in LDS and two more on their way in registers.  While a stage is computed, the
+// next one goes from registers into the other buffer and the one three ahead is fetched, piece by piece between the MFMAs, so a
+// stage costs one barrier and no wave ever waits for staging alone; k runs upwards in pairs as in gemm_lds_kernel.
+//   k-contiguous operand: a row's even k, then its odd k (lane half h of an MFMA takes k = 2 s + h), pitch 36: one 16-byte LDS read
+//                         feeds four MFMA steps; 16 rows of a read cover all banks.
+//   row-contiguous operand: S[k][r] as above, one 4-byte read per step.
+// Bound by the matrix pipe.  Measured (f32, NN / NT / TN / TT, TFLOP/s; in brackets one 64-deep stage per block, computing and staging in
+// turns, as before): 4096 x 1024 x 4096 131 / 134 / 134 / 138 (117 / 123 / 125 / 121), 4096 x 4096 x 1024 132 / 133 / 133 / 134
+// (124 / 125 / 127 / 126), 2048^3 128 / 134 / 131 / 134 (116 / 120 / 122 / 119); 4096^3 138 to 140 of 157.
+constexpr int KP = 32, PP = KP + 4;
+template <int TN, bool TA, bool TB> constexpr int pipe_stage_floats() { return (TA ? KP * 128 : 128 * PP) + (TB ? 32 * TN * PP : KP * 32 * TN); }
+template <int TN, bool TA, bool TB, int EP, bool KT = false>
+__global__ __launch_bounds__(NT, 2) void gemm_pipe_kernel(const Params p) {
+    static_assert(!KT || (!TA && TB), "the K tail is handled for k-contiguous operands");
+    constexpr int BM = 128, BN = 32 * TN;
+    constexpr int ASZ = TA ? KP * BM : BM * PP, STAGE = pipe_stage_floats<TN, TA, TB>();
+    constexpr int NA = BM * KP / 4 / NT, NB = BN * KP / 4 / NT;  // float4 per thread per stage
+    FX_DYNAMIC_SMEM(float, smem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+    const float* const Ab = p.A + (i64)blockIdx.y * p.sa;
+    const float* const Bb = p.B + (i64)blockIdx.y * p.sb;
+    float* const Cb = p.C + (i64)blockIdx.y * p.sc;
+    int tile = blockIdx.x;
+    if (p.xcd_chunk) tile = (tile & 7) * p.xcd_chunk + (tile >> 3);
+    const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+    const int m0 = tm * BM, n0 = tn * BN;
+
+    f32x16 acc[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) turn[igemm::Mfma<float>::row(e, lane) * WC + j * 32 + l32] = acc[j][e];
-        __syncthreads();
-        const int n = n0 + wn * WC + 4 * (lane % CG), left = p.N - n;
-        float bias[4] = {0.f, 0.f, 0.f, 0.f};
-        if (p.ex.bias) {
+        for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+
+    // staging maps.  k-contiguous: thread t owns float4 t % 8 (k = 4 (t % 8) ..) of rows t / 8 + 32 u; row-contiguous, R floats per k:
+    // float4 t % (R / 4) of k rows t / (R / 4) + (NT / (R / 4)) u.  Rows past the matrix re-read its last row.
+    uint32_t a_off[NA], b_off[NB];
+    if (!TA) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q < left) bias[q] = p.ex.bias[n + q];
+        for (int u = 0; u < NA; ++u) a_off[u] = (uint32_t)((i64)min(m0 + (tid >> 3) + 32 * u, p.M - 1) * p.lda + 4 * (tid & 7)) * 4u;
+    } else {
+        constexpr int Q = BM / 4, RS = NT / Q;
+        const int c4 = min(m0 + 4 * (tid % Q), p.M - 4);
+#pragma unroll
+        for (int u = 0; u < NA; ++u) a_off[u] = (uint32_t)((i64)(tid / Q + RS * u) * p.lda + c4) * 4u;
+    }
+    if (TB) {
+#pragma unroll
+        for (int u = 0; u < NB; ++u) b_off[u] = (uint32_t)((i64)min(n0 + (tid >> 3) + 32 * u, p.N - 1) * p.ldb + 4 * (tid & 7)) * 4u;
+    } else {
+        constexpr int Q = BN / 4, RS = NT / Q;
+        const int c4 = min(n0 + 4 * (tid % Q), p.N - 4);
+#pragma unroll
+        for (int u = 0; u < NB; ++u) b_off[u] = (uint32_t)((i64)(tid / Q + RS * u) * p.ldb + c4) * 4u;
+    }
+    typedef float f32x4 __attribute__((ext_vector_type(4)));  // one value for the compiler, not four: it stays in its four registers
+    f32x4 v[2][NA + NB];            // two stages on their way
+    bool past[2] = {false, false};  // KT: this thread's four k of the stage lie past K (its loads re-read the stage's first vector)
+    // unit u of a stage's staging: one 16-byte load, and later its way into LDS
+    auto fetch = [&](int set, int k0, int u) __attribute__((always_inline)) {
+        uint32_t back = 0;
+        if constexpr (KT) {
+            past[set] = k0 + 4 * (tid & 7) >= p.K;
+            back = past[set] ? 16u * (tid & 7) : 0u;
         }
-#pragma unroll 1
-        for (int r = lane / CG; r < 32; r += RPI) {
-            const int m = m0 + wm * 32 + r;
-            if (m >= p.M || left <= 0) continue;
-            const i64 i = (i64)m * p.N + n;
-            const float4 t4 = *reinterpret_cast<const float4*>(turn + r * WC + 4 * (lane % CG));
-            float v[4] = {t4.x, t4.y, t4.z, t4.w}, res[4] = {0.f, 0.f, 0.f, 0.f};
-            typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // a row of C starts at any element
-            if (p.ex.residual) {
-                if (left >= 4) {
-                    const f4u q4 = *reinterpret_cast<const f4u*>(p.ex.residual + i);
-                    res[0] = q4.x; res[1] = q4.y; res[2] = q4.z; res[3] = q4.w;
-                } else {
+        const float* const base = u < NA ? (TA ? Ab + (i64)k0 * p.lda : Ab + k0) : (TB ? Bb + k0 : Bb + (i64)k0 * p.ldb);
+        const uint32_t off = u < NA ? a_off[u < NA ? u : 0] : b_off[u < NA ? 0 : u - NA];
+        v[set][u] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(base) + (off - back));
+    };
+    auto park = [&](int set, int buf, int u) __attribute__((always_inline)) {
+        f32x4& x = v[set][u];
+        // the loaded values are first touched here: left alone, the compiler rearranges them for the write right behind the load and
+        // waits for memory there
+        FX_PIN_VGPR(x);
+        if constexpr (KT) {
+            if (past[set]) x = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const bool is_a = u < NA, kc = is_a ? !TA : TB;  // k-contiguous: even k, then odd k
+        const int R = is_a ? BM : BN, Q = R / 4, w = is_a ? u : u - NA;
+        float* const d = smem + buf * STAGE + (is_a ? 0 : ASZ);
+        if (kc) {
+            float* const r = d + ((tid >> 3) + 32 * w) * PP + 2 * (tid & 7);
+            *reinterpret_cast<float2*>(r) = make_float2(x.x, x.z);
+            *reinterpret_cast<float2*>(r + KP / 2) = make_float2(x.y, x.w);
+        } else {
+            *reinterpret_cast<f32x4*>(d + (tid / Q + NT / Q * w) * R + 4 * (tid % Q)) = x;
+        }
+    };
+
+    // operands of four MFMA steps (group g: steps 4 g .. 4 g + 3)
+    const float* const ar = TA ? smem + half * BM + wave * 32 + l32 : smem + (wave * 32 + l32) * PP + half * (KP / 2);
+    const float* const br = TB ? smem + ASZ + l32 * PP + half * (KP / 2) : smem + ASZ + half * BN + l32;
+    auto read = [&](float (&a)[4], float (&b)[TN][4], int buf, int g) __attribute__((always_inline)) {
+        const float* const x = ar + buf * STAGE;
+        const float* const y = br + buf * STAGE;
+        if (TA) {
 #pragma unroll
-                    for (int q = 0; q < 3; ++q)
-                        if (q < left) res[q] = p.ex.residual[i + q];
-                }
-            }
+            for (int q = 0; q < 4; ++q) a[q] = x[2 * (4 * g + q) * BM];
+        } else {
+            const float4 v = *reinterpret_cast<const float4*>(x + 4 * g);
+            a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
+        }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (p.ex.bias) v[q] = v[q] + bias[q];
-            if (p.ex.pre) {
-                if (left >= 4) {
-                    *reinterpret_cast<f4u*>(p.ex.pre + i) = f4u{v[0], v[1], v[2], v[3]};
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 3; ++q)
-                        if (q < left) p.ex.pre[i + q] = v[q];
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                v[q] = fxact::apply<float>(p.ex.act, v[q]);
-                if (p.ex.residual) v[q] = v[q] + res[q];
-            }
-            if (left >= 4) {
-                *reinterpret_cast<f4u*>(Cb + i) = f4u{v[0], v[1], v[2], v[3]};
+        for (int j = 0; j < TN; ++j) {
+            if (TB) {
+                const float4 v = *reinterpret_cast<const float4*>(y + j * 32 * PP + 4 * g);
+                b[j][0] = v.x; b[j][1] = v.y; b[j][2] = v.z; b[j][3] = v.w;
             } else {
 #pragma unroll
-                for (int q = 0; q < 3; ++q)
-                    if (q < left) Cb[i + q] = v[q];
+                for (int q = 0; q < 4; ++q) b[j][q] = y[2 * (4 * g + q) * BN + j * 32];
             }
         }
-        return;
-    }
-    constexpr bool BIAS = EP == EP_BIAS;
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // One step's MFMAs, then what `between` puts behind them: the matrix pipe works for 64 cycles per instruction, staging slips in.
+    auto mma = [&](const float (&a)[4], const float (&b)[TN][4], auto&& between) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int n = n0 + (wn * TN + j) * 32 + l32;
-        const float bj = BIAS && !p.bias_per_row ? p.bias[n < p.N ? n : p.N - 1] : 0.f;
-        if (n < p.N) {
+        for (int q = 0; q < 4; ++q) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = m0 + wm * 32 + igemm::Mfma<float>::row(e, lane);
-                if (m < p.M) {
-                    float v = acc[j][e];
-                    if (BIAS) {
-                        v = v + (p.bias_per_row ? p.bias[m] : bj);
-                        if (p.relu) v = v > 0.f ? v : 0.f;
-                    }
-                    Cb[(i64)m * p.N + n] = v;
-                }
-            }
+            for (int j = 0; j < TN; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[q], b[j][q], acc[j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            between(q);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    float a0[4], b0[TN][4], a1[4], b1[TN][4];
+    // One stage, in buffer `buf`, whose first group is in (a0, b0).  Set `set` holds the next stage, which goes into the other buffer
+    // (last read in the stage before this one, which every wave has left through the barrier below), and takes the third one from here.
+    // The barrier comes before the last group: its MFMAs cover the first reads of the next stage.  Nothing here is conditional -- past
+    // the end the last stage is loaded once more, parked and never read -- since a branch around a load makes its result a copy of the
+    // loaded registers, and the copy waits for memory on the spot.
+    constexpr int UNITS = NA + NB, PER = (UNITS + 7) / 8;
+    const int k_last = (p.K - 1) / KP * KP;
+    auto stage = [&](int k0, int set, int buf) __attribute__((always_inline)) {
+        const int k3 = min(k0 + 3 * KP, k_last);
+        auto put = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = s * PER; u < (s + 1) * PER && u < UNITS; ++u) park(set, buf ^ 1, u);
+        };
+        read(a1, b1, buf, 1);
+        mma(a0, b0, [&](int q) __attribute__((always_inline)) { put(q); });
+        read(a0, b0, buf, 2);
+        mma(a1, b1, [&](int q) __attribute__((always_inline)) { put(4 + q); });
+        read(a1, b1, buf, 3);
+        mma(a0, b0, [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = q * 2 * PER; u < (q + 1) * 2 * PER && u < UNITS; ++u) fetch(set, k3, u);
+        });
+        __syncthreads();
+        read(a0, b0, buf ^ 1, 0);
+        mma(a1, b1, [](int) {});
+    };
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) fetch(0, 0, u);
+    __builtin_amdgcn_sched_barrier(0);  // the loads in the order in which the loop waits for them
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) fetch(1, min(KP, k_last), u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) park(0, 0, u);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) fetch(0, min(2 * KP, k_last), u);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    read(a0, b0, 0, 0);
+    int k0 = 0;
+    for (; k0 + KP < p.K; k0 += 2 * KP) {
+        stage(k0, 1, 0);
+        stage(k0 + KP, 0, 1);
     }
+    if constexpr (KT) {
+        if (k0 < p.K) stage(k0, 1, 0);  // an odd number of stages (without a tail K is a multiple of two)
+    }
+    if constexpr (EP == EP_FULL) __syncthreads();  // the turn through LDS below: the last stage's readers are all through
+    store_tile<TN, EP>(p, Cb, smem, acc, m0 + wave * 32, n0, lane, wave);
 }
 
 struct Plan {
@@ -381,10 +537,26 @@ inline Plan make_plan(int num_cus, bool ta, bool tb, i64 M, i64 N, i64 K, i64 ld
     pl.tiles_n = (int)fx::ceil_div(N, (i64)pl.bn());
     const i64 a_span = ta ? (i64)KC * lda + M : (i64)M * lda, b_span = tb ? (i64)N * ldb : (i64)KC * ldb + N;
     if (a_span * 4 >= (1ll << 32) || b_span * 4 >= (1ll << 32)) return pl;
-    pl.smem = (size_t)((ta ? KC * pl.bm() : pl.bm() * PK) + (tb ? pl.bn() * PK : KC * pl.bn())) * sizeof(float) * (pl.WM == 2 ? 2 : 1);
-    if (pl.smem > (pl.WM == 2 ? LDS_BUDGET_MID : LDS_BUDGET)) return pl;
+    if (pl.WM == 2) {  // (the 128-row tiles' LDS goes by their template arguments)
+        pl.smem = (size_t)((ta ? KC * pl.bm() : pl.bm() * PK) + (tb ? pl.bn() * PK : KC * pl.bn())) * sizeof(float) * 2;
+        if (pl.smem > LDS_BUDGET_MID) return pl;
+    }
     pl.ok = true;
     return pl;
+}
+
+template <int TN, bool TA, bool TB, int EP, bool KT> inline int launch_pipe_ep(fx_ctx* c, const Params& p, dim3 grid, dim3 blk) {
+    constexpr size_t lds = 2 * sizeof(float) * pipe_stage_floats<TN, TA, TB>();
+    static const hipError_t attr = hipFuncSetAttribute((const void*)gemm_pipe_kernel<TN, TA, TB, EP, KT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    FX_HIP_CHECK(attr);
+    FX_LAUNCH(grid, blk, lds, c->stream, (p), gemm_pipe_kernel<TN, TA, TB, EP, KT>);
+    FX_LAUNCH_CHECK();
+    return FX_OK;
+}
+template <int TN, bool TA, bool TB, bool KT> inline int launch_pipe(fx_ctx* c, const Params& p, dim3 grid, dim3 blk) {
+    if (p.ex.any()) return launch_pipe_ep<TN, TA, TB, EP_FULL, KT>(c, p, grid, blk);
+    if (p.bias) return launch_pipe_ep<TN, TA, TB, EP_BIAS, KT>(c, p, grid, blk);
+    return launch_pipe_ep<TN, TA, TB, EP_NONE, KT>(c, p, grid, blk);
 }
 
 template <int TN, int WM, bool TA, bool TB, bool KT = false>
@@ -393,22 +565,26 @@ inline int launch(fx_ctx* c, const Plan& pl, const Params& p, int batch) {
     if constexpr (!KT && !TA && TB) {
         if (p.K % KC != 0) return launch<TN, WM, TA, TB, true>(c, pl, p, batch);
     }
-    constexpr int budget = (int)(WM == 2 ? LDS_BUDGET_MID : LDS_BUDGET);
-    static const hipError_t attr0 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, EP_NONE, KT>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, budget);
-    static const hipError_t attr1 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, EP_BIAS, KT>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, budget);
-    FX_HIP_CHECK(attr0);
-    FX_HIP_CHECK(attr1);
-    if (p.ex.any()) {
-        static const hipError_t attr2 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, WM, TA, TB, EP_FULL, KT>,
+    if constexpr (WM == 4) {
+        return launch_pipe<TN, TA, TB, KT>(c, p, grid, blk);
+    } else {
+        constexpr int budget = (int)LDS_BUDGET_MID;
+        static const hipError_t attr0 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, TA, TB, EP_NONE, KT>,
                                                             hipFuncAttributeMaxDynamicSharedMemorySize, budget);
-        FX_HIP_CHECK(attr2);
-        FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, EP_FULL, KT>);
-    } else if (p.bias) FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, EP_BIAS, KT>);
-    else FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, WM, TA, TB, EP_NONE, KT>);
-    FX_LAUNCH_CHECK();
-    return FX_OK;
+        static const hipError_t attr1 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, TA, TB, EP_BIAS, KT>,
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, budget);
+        FX_HIP_CHECK(attr0);
+        FX_HIP_CHECK(attr1);
+        if (p.ex.any()) {
+            static const hipError_t attr2 = hipFuncSetAttribute((const void*)gemm_lds_kernel<TN, TA, TB, EP_FULL, KT>,
+                                                                hipFuncAttributeMaxDynamicSharedMemorySize, budget);
+            FX_HIP_CHECK(attr2);
+            FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, TA, TB, EP_FULL, KT>);
+        } else if (p.bias) FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, TA, TB, EP_BIAS, KT>);
+        else FX_LAUNCH(grid, blk, pl.smem, c->stream, (p), gemm_lds_kernel<TN, TA, TB, EP_NONE, KT>);
+        FX_LAUNCH_CHECK();
+        return FX_OK;
+    }
 }
 template <bool TA, bool TB>
 inline int launch_tn(fx_ctx* c, const Plan& pl, const Params& p, int batch) {
