@@ -21,35 +21,36 @@ namespace {
 using namespace vio;
 
 // ---- lookup --------------------------------------------------------------------------------------------------------------------
-// One thread per vector of the output, U of them a block apart; rows of nv vectors.
+// One thread per vector of the output, U of them a block apart; a row has nv vectors, the last of which may be incomplete.  All loads of
+// the ids, then all loads of the table are in flight together: a token outside the table reads row 0 and stores zeros.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict__ W, const int64_t* __restrict__ ids, T* __restrict__ out, i64 total,
-                                                            unsigned nv, i64 vocab, T scale) {
+                                                            unsigned nv, i64 vocab, int D, T scale) {
     constexpr int U = 4;
     const i64 first = (i64)blockIdx.x * (256 * U);
     const i64 row0 = first / nv;  // block-uniform
-    const unsigned off = (unsigned)(first - row0 * nv);
+    const unsigned off = (unsigned)(first - row0 * nv), last = (unsigned)(min(total - first, (i64)(256 * U)) - 1);
+    unsigned dr[U], col[U];
+    i64 id[U];
     T v[U][V];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const i64 i = first + u * 256 + threadIdx.x;
-        const unsigned q = off + u * 256 + threadIdx.x, dr = q / nv, col = q - dr * nv;
-        i64 id = -1;
-        if (i < total) id = ids[row0 + dr];
-        if (id >= 0 && id < vocab) {
-            load<V>(W + (id * nv + col) * V, v[u]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[u][e] = T(0);
-        }
+        const unsigned q = off + min(u * 256 + threadIdx.x, last);  // past the end: the last vector again, not stored
+        dr[u] = q / nv;
+        col[u] = (q - dr[u] * nv) * V;
+        id[u] = ids[row0 + dr[u]];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const i64 i = first + u * 256 + threadIdx.x;
-        if (i < total) {
+        if (id[u] < 0 || id[u] >= vocab) id[u] = -1;
+        load_part<V>(W + (id[u] < 0 ? 0 : id[u]) * D, (int)col[u], D, v[u]);
+    }
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[u][e] = v[u][e] * scale;
-            store<V>(out + i * V, v[u]);
+    for (int u = 0; u < U; ++u) {
+        if (u * 256 + threadIdx.x <= last) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[u][e] = id[u] < 0 ? T(0) : v[u][e] * scale;
+            store_part<V>(out + (row0 + dr[u]) * D, (int)col[u], D, v[u]);
         }
     }
 }
@@ -376,10 +377,15 @@ __global__ __launch_bounds__(256) void embedding_add_kernel(const T* __restrict_
         for (int u = 0; u < V; ++u) zero[u] = T(0);
         // all 256 threads run over (row, vector) pairs of this block's column range
         const i64 c0 = (i64)blockIdx.y * (V << a.tpp_log), c1 = min(a.D, c0 + (V << a.tpp_log));
-        const int nv = (int)((c1 - c0) / V);
+        const int nv = (int)((c1 - c0 + V - 1) / V);
         for (int i = threadIdx.x; i < ZROWS * nv; i += 256) {
             const int r = i / nv;
-            if (!present[r]) store_stream<V>(dW + (v0 + r) * a.D + c0 + (i64)(i - r * nv) * V, zero);
+            if (!present[r]) {
+                const int j = (int)c0 + (i - r * nv) * V;
+                T* const row = dW + (v0 + r) * a.D;
+                if (j + V <= a.D) store_stream<V>(row + j, zero);
+                else store_part<V>(row, j, (int)a.D, zero);
+            }
         }
         return;
     }
@@ -400,7 +406,7 @@ __global__ __launch_bounds__(256) void embedding_add_kernel(const T* __restrict_
         for (int j = 0; j < U; ++j) {
             const i64 at = min(p + j, p1 - 1);
             k[j] = keys[at];
-            load<V>(g + (i64)pos[at] * a.D + col, v[j]);
+            load_part<V>(g + (i64)pos[at] * a.D, (int)col, (int)a.D, v[j]);
         }
         const i64 behind = min(p + U, p1);
         k[U] = behind < a.n ? keys[behind] : 0xffffffffu;
@@ -415,11 +421,11 @@ __global__ __launch_bounds__(256) void embedding_add_kernel(const T* __restrict_
                 if (ends || last) {
                     if (k[j] < (uint32_t)a.vocab) {
                         if (open || !ends) {
-                            store<V>(edge + (piece * 2 + (open ? 0 : (k[j] == keys[p0] ? 0 : 1))) * a.D + col, acc);
+                            store_part<V>(edge + (piece * 2 + (open ? 0 : (k[j] == keys[p0] ? 0 : 1))) * a.D, (int)col, (int)a.D, acc);
                         } else {
 #pragma unroll
                             for (int u = 0; u < V; ++u) acc[u] = acc[u] * scale;
-                            store<V>(dW + (i64)k[j] * a.D + col, acc);
+                            store_part<V>(dW + (i64)k[j] * a.D, (int)col, (int)a.D, acc);
                         }
                     }
 #pragma unroll
@@ -467,7 +473,7 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t* __r
             for (int j = 0; j < U; ++j) {
                 const i64 piece = q + 4 * j;
                 if (piece <= end) {
-                    load<V>(edge + (piece * 2 + (piece == b && !whole ? 1 : 0)) * a.D + col, v[j]);
+                    load_part<V>(edge + (piece * 2 + (piece == b && !whole ? 1 : 0)) * a.D, (int)col, (int)a.D, v[j]);
                 } else {
 #pragma unroll
                     for (int u = 0; u < V; ++u) v[j][u] = T(0);
@@ -489,7 +495,7 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t* __r
             for (int w = 1; w < 4; ++w) s = s + sm[w][lane * V + u];
             acc[u] = s * scale;
         }
-        store<V>(dW + (i64)k * a.D + col, acc);
+        store_part<V>(dW + (i64)k * a.D, (int)col, (int)a.D, acc);
     }
 }
 
@@ -509,11 +515,9 @@ int embedding_fwd(fx_ctx* c, const T* W, const int64_t* ids, T* out, i64 n, i64 
     FX_REQUIRE(W && ids && out, "fx_embedding_fwd: null pointer");
     FX_REQUIRE(!fx::overlap(out, n * D, W, vocab * D), "fx_embedding_fwd: the output overlaps the table");
     constexpr int V = 16 / (int)sizeof(T);
-    const bool vec = D % V == 0 && fx::aligned16(W) && fx::aligned16(out);
-    const i64 nv = vec ? D / V : D, total = n * nv, blocks = fx::ceil_div(total, (i64)1024);
+    const i64 nv = fx::ceil_div(D, (i64)V), total = n * nv, blocks = fx::ceil_div(total, (i64)1024);
     FX_REQUIRE(blocks <= 0x7fffffff, "fx_embedding_fwd: too many elements");
-    if (vec) FX_LAUNCH(dim3((unsigned)blocks), dim3(256), 0, c->stream, (W, ids, out, total, (unsigned)nv, vocab, scale), embedding_fwd_kernel<T, V>);
-    else FX_LAUNCH(dim3((unsigned)blocks), dim3(256), 0, c->stream, (W, ids, out, total, (unsigned)nv, vocab, scale), embedding_fwd_kernel<T, 1>);
+    FX_LAUNCH(dim3((unsigned)blocks), dim3(256), 0, c->stream, (W, ids, out, total, (unsigned)nv, vocab, (int)D, scale), embedding_fwd_kernel<T, V>);
     FX_LAUNCH_CHECK();
     return FX_OK;
 }
@@ -597,8 +601,7 @@ int embedding_bwd(fx_ctx* c, const T* g, const int64_t* ids, T* dW, i64 n, i64 v
         }
     }
     T* edge = (T*)(scratch + edge_at);
-    const bool vec = D % V == 0 && fx::aligned16(g) && fx::aligned16(dW);
-    return vec ? add_and_join<T, V>(c, g, keys, pos, dW, edge, scale, a) : add_and_join<T, 1>(c, g, keys, pos, dW, edge, scale, a);
+    return add_and_join<T, V>(c, g, keys, pos, dW, edge, scale, a);
 }
 }  // namespace
 

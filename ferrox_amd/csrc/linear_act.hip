@@ -32,9 +32,9 @@ __global__ __launch_bounds__(64 * GROUPS) void act_bwd_kernel(const T* dy, const
             T g[U][V], p[U][V];
 #pragma unroll
             for (int q = 0; q < U; ++q) {
-                const i64 at = min(r + q * step, rows - 1) * cols + c;
-                load<V>(dy + at, g[q]);
-                load<V>(pre + at, p[q]);
+                const i64 at = min(r + q * step, rows - 1) * cols;
+                load_part<V>(dy + at, (int)c, (int)cols, g[q]);
+                load_part<V>(pre + at, (int)c, (int)cols, p[q]);
             }
 #pragma unroll
             for (int q = 0; q < U; ++q) {
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64 * GROUPS) void act_bwd_kernel(const T* dy, const
                         g[q][u] = g[q][u] * fxact::grad<T, ACT>(p[q][u]);
                         s[u] = s[u] + g[q][u];
                     }
-                    store<V>(dpre + (r + q * step) * cols + c, g[q]);
+                    store_part<V>(dpre + (r + q * step) * cols, (int)c, (int)cols, g[q]);
                 }
             }
         }
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * GROUPS) void act_bwd_kernel(const T* dy, const
 #pragma unroll
         for (int u = 0; u < V; ++u)
             for (int w = 1; w < GROUPS; ++w) s[u] = s[u] + sm[w][lane * V + u];
-        store<V>(part + (i64)blockIdx.y * cols + c, s);
+        store_part<V>(part + (i64)blockIdx.y * cols, (int)c, (int)cols, s);
     }
 }
 
@@ -112,8 +112,7 @@ int linear_act_bwd(fx_ctx* c, i64 B, i64 in, i64 out, const T* dY, const T* W, c
     {
         std::lock_guard<std::mutex> lk(c->launch_mutex);
         constexpr int V = 16 / (int)sizeof(T);
-        const bool vec = out % V == 0 && fx::aligned16(dY) && fx::aligned16(pre) && fx::aligned16(dpre) && (!db || fx::aligned16(db));
-        const int rc = vec ? launch_act_bwd<T, V>(c, act, dY, pre, dpre, db, B, out) : launch_act_bwd<T, 1>(c, act, dY, pre, dpre, db, B, out);
+        const int rc = launch_act_bwd<T, V>(c, act, dY, pre, dpre, db, B, out);
         if (rc) return rc;
     }
     return Products<T>::bwd(c, B, in, out, dpre, W, X, dX, dW);
