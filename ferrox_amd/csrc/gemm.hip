@@ -8,6 +8,7 @@
 #include "gemm_thin.hpp"
 #include "gemm_small.hpp"
 #include "gemm_epilogue.hpp"
+#include "gemm_rows.hpp"
 
 extern "C" int fx_bias_act_f32(fx_ctx*, float*, const float*, int64_t, int64_t, int64_t, int);
 extern "C" int fx_bias_act_f64(fx_ctx*, double*, const double*, int64_t, int64_t, int64_t, int);
@@ -249,6 +250,10 @@ int gemm_bias_act_residual(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const
         std::lock_guard<std::mutex> lk(c->launch_mutex);
         if (int rc = launch_zero<T>(c, C, n)) return rc;
         return ex.any() ? gep::launch_pass<T>(c, C, n, N, ex) : FX_OK;
+    }
+    if (grows::eligible(ta != 0, tb != 0, M, K)) {
+        std::lock_guard<std::mutex> lk(c->launch_mutex);
+        return grows::run<T>(c, M, N, K, A, B, C, ex);
     }
     // what fx_gemm_bias_act does already goes its way, same kernels and bits
     if (bias && !residual && !pre && act <= fxact::RELU) return gemm<T>(c, ta, tb, M, N, K, A, B, C, bias, act);
