@@ -513,7 +513,8 @@ int embedding_fwd(fx_ctx* c, const T* W, const int64_t* ids, T* out, i64 n, i64 
     if (int rc = check<T>(c, "fx_embedding_fwd", n, vocab, D)) return rc;
     if (n == 0) return FX_OK;
     FX_REQUIRE(W && ids && out, "fx_embedding_fwd: null pointer");
-    FX_REQUIRE(!fx::overlap(out, n * D, W, vocab * D), "fx_embedding_fwd: the output overlaps the table");
+    FX_REQUIRE(!fx::overlap(out, n * D, W, vocab * D) && !fx::overlap((const char*)out, n * D * (i64)sizeof(T), (const char*)ids, n * 8),
+               "fx_embedding_fwd: the output overlaps an input");
     constexpr int V = 16 / (int)sizeof(T);
     const i64 nv = fx::ceil_div(D, (i64)V), total = n * nv, blocks = fx::ceil_div(total, (i64)1024);
     FX_REQUIRE(blocks <= 0x7fffffff, "fx_embedding_fwd: too many elements");
@@ -552,7 +553,8 @@ template <typename T>
 int embedding_bwd(fx_ctx* c, const T* g, const int64_t* ids, T* dW, i64 n, i64 vocab, i64 D, T scale) {
     if (int rc = check<T>(c, "fx_embedding_bwd", n, vocab, D)) return rc;
     FX_REQUIRE(dW && (n == 0 || (g && ids)), "fx_embedding_bwd: null pointer");
-    FX_REQUIRE(!fx::overlap(dW, vocab * D, g, n * D), "fx_embedding_bwd: the output overlaps the gradient");
+    FX_REQUIRE(!fx::overlap(dW, vocab * D, g, n * D) && !fx::overlap((const char*)dW, vocab * D * (i64)sizeof(T), (const char*)ids, n * 8),
+               "fx_embedding_bwd: the output overlaps an input");
     std::lock_guard<std::mutex> lk(c->launch_mutex);
     constexpr int V = 16 / (int)sizeof(T);
     Add a;
@@ -566,9 +568,11 @@ int embedding_bwd(fx_ctx* c, const T* g, const int64_t* ids, T* dW, i64 n, i64 v
     a.tpp_log = 0;
     int passes = 1;
     while (passes < 4 && (vocab >> (BITS * passes)) != 0) ++passes;  // the largest key is vocab itself
-    // the one-launch sort while the blocks' reading of all tokens, 8 bytes each, stays below 128 MB (about 15 us from the L2s): up to
-    // 32768 tokens of 131000 ids, 4096 of a million
-    const bool small = n <= RANGE_MAX && n * (vocab / BINS + 1) <= (1ll << 24);
+    // the one-launch sort while its blocks are few and what they read together, 8 bytes per token each, stays below 128 MB.  Whole call,
+    // rows of 8 floats, against the tiled passes (us): 16000 tokens of 30000 ids 24.6 / 42.4, of 260000 44 / 60, 32000 of 130000 40 / 62,
+    // 4000 of a million 64 / 73, 300 of 200000 16.5 / 39, 100 of four million 107 / 104.
+    const i64 ranges = vocab / BINS + 1;
+    const bool small = n <= RANGE_MAX && ranges <= 8192 && n * ranges <= (1ll << 24);
     const i64 tiles = fx::ceil_div(n, (i64)TILE), entries = tiles * BINS;
     // scratch: [keys][pos] once or twice, the table of counts, the partial rows
     const i64 nkeys = fx::ceil_div(n, (i64)64) * 64, lists = small ? 2 : 4;

@@ -157,24 +157,24 @@ int fill_table(Tensors<T>& tt, int base, int count, const T* const* g, T* const*
     return k;
 }
 
-// No output may share memory with another tensor of the call (its own gradient, exactly, excepted).
+// No output (the norm is one) may share memory with another tensor of the call (its own gradient, exactly, excepted).
 template <typename T>
-int check_overlaps(int count, const T* const* g, T* const* out, const int64_t* n, const T* norm) {
+int check_overlaps(int count, const T* const* g, T* const* out, const int64_t* n, const T* norm, const char* what) {
     struct Span { uintptr_t lo, hi; int k; bool out; };
     std::vector<Span> spans;
     spans.reserve(2 * (size_t)count + 1);
     for (int k = 0; k < count; ++k) {
         if (n[k] == 0) continue;
         const uintptr_t bytes = (uintptr_t)n[k] * sizeof(T);
-        spans.push_back({(uintptr_t)out[k], (uintptr_t)out[k] + bytes, k, true});
-        if (g[k] != out[k]) spans.push_back({(uintptr_t)g[k], (uintptr_t)g[k] + bytes, k, false});
+        if (out) spans.push_back({(uintptr_t)out[k], (uintptr_t)out[k] + bytes, k, true});
+        if (!out || g[k] != out[k]) spans.push_back({(uintptr_t)g[k], (uintptr_t)g[k] + bytes, k, false});
     }
     spans.push_back({(uintptr_t)norm, (uintptr_t)norm + sizeof(T), count, true});
     std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
     // walking up: the furthest end of the outputs so far, and of everything so far
     uintptr_t out_end = 0, any_end = 0;
     for (const Span& s : spans) {
-        FX_REQUIRE(!(s.lo < out_end || (s.out && s.lo < any_end)), "fx_clip_grad_norm_multi: an output overlaps another tensor of the call (tensor %d)", s.k);
+        FX_REQUIRE(!(s.lo < out_end || (s.out && s.lo < any_end)), "%s: an output overlaps another tensor of the call (at tensor %d)", what, s.k);
         any_end = std::max(any_end, s.hi);
         if (s.out) out_end = std::max(out_end, s.hi);
     }
@@ -193,9 +193,7 @@ int grad_norm(fx_ctx* c, int count, const T* const* g, T* const* out, const int6
         FX_REQUIRE(n[k] <= (i64)0x7fffffff * CHUNK, "%s: too many elements in tensor %d", what, k);
         FX_REQUIRE(n[k] == 0 || (g[k] && (!out || out[k])), "%s: null pointer in tensor %d", what, k);
     }
-    if (out) {
-        if (int rc = check_overlaps<T>(count, g, out, n, norm)) return rc;
-    }
+    if (int rc = check_overlaps<T>(count, g, out, n, norm, what)) return rc;
     std::lock_guard<std::mutex> lk(c->launch_mutex);
     Tensors<T> tt;
     // launches of at most TABLE tensors each; together they leave at most about MAX_PARTIALS partial sums

@@ -36,6 +36,11 @@ def shifted(ctx, a, by=1):
     return v
 
 
+def _view(ctx, ptr, shape, dtype=np.float32):
+    from ferrox_amd import capi
+    return capi.DeviceArray(ctx, shape, dtype, ptr, 0, None)
+
+
 def filled(ctx, shape, dtype, by=0):
     """An output full of NaN between guard elements, and a check that the guards are untouched."""
     n = int(np.prod(shape))
@@ -73,7 +78,7 @@ EMBED = [(1, 1, 1, "zipf"), (1, 300, 8, "zipf"), (5, 7, 3, "outside"), (16, 2, 6
          (33, 1000, 260, "each"), (64, 255, 16, "each"), (65, 256, 16, "each"), (700, 257, 36, "outside"), (1024, 65536, 4, "zipf"),
          (1025, 70, 1001, "zipf"), (2048, 3, 128, "zipf"), (4097, 40, 20, "padding"), (4096, 500, 40, "one"), (5000, 65535, 7, "outside"),
          (16384, 5000, 24, "zipf"), (16385, 5000, 24, "zipf"), (20000, 300, 33, "outside"), (40001, 70000, 8, "zipf"), (70000, 1, 5, "one"),
-         (100, 50, 5000, "zipf"), (66000, 17000000, 1, "zipf")]
+         (100, 50, 5000, "zipf"), (300, 2200000, 2, "zipf"), (2000, 600000, 3, "outside"), (32768, 300, 4, "zipf"), (32768, 200, 3, "one"), (66000, 17000000, 1, "zipf")]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -208,7 +213,7 @@ def test_rmsnorm_in_place_and_unaligned(ctx, rows, dim, dtype):
 # ---- Linear with activation and residual -------------------------------------------------------------------------------------------------
 LINEAR = [(1, 1, 1), (1, 32, 8), (5, 7, 3), (33, 31, 65), (64, 64, 64), (100, 64, 100), (256, 784, 256), (256, 256, 10), (10, 2048, 300), (128, 132, 128),
           (130, 192, 260), (16, 4096, 40), (300, 1000, 129), (512, 128, 1024), (1024, 512, 512), (2, 20000, 6), (256, 16384, 10), (32, 64, 9000),
-          (1030, 260, 1028)]
+          (1030, 260, 1028), (2100, 40, 2100), (1, 4097, 130), (2, 513, 31), (3, 1001, 257), (4, 512, 64), (4, 2600, 5)]
 ACTS = ["none", "relu", "gelu", "silu"]
 
 
@@ -263,6 +268,25 @@ def test_gemm_epilogue_unaligned_empty_and_plain(ctx, dtype):
     # K = 0: the empty product, still with its epilogue
     check(getattr(lib, f"fx_gemm_bias_act_residual_{s}")(ctx.h, 0, 0, 70, 96, 0, None, None, ctx.upload(bias).ptr, None, None, out.ptr, 1))
     assert np.array_equal(out.numpy(), np.broadcast_to(np.maximum(bias, 0), (70, 96))) and oi()
+
+
+@pytest.mark.parametrize("m,k,n", [(2052, 192, 2048), (2560, 128, 2564), (2049, 132, 2053), (1024, 256, 512), (1025, 260, 511)])
+def test_gemm_epilogue_of_the_large_tiles(ctx, m, k, n):
+    """f32 products of the 128- and 64-row tiles, with and without a remainder of K, rows of C at any alignment."""
+    rng = np.random.default_rng(m)
+    A, B = rng.standard_normal((m, k)).astype(np.float32), (rng.standard_normal((k, n)) / np.sqrt(k)).astype(np.float32)
+    bias, res = rng.standard_normal(n).astype(np.float32), rng.standard_normal((m, n)).astype(np.float32)
+    dbias, dres = shifted(ctx, bias), shifted(ctx, res, 3)
+    for (ta, tb), act, use in zip(((False, True), (False, False), (True, False), (True, True)), ("gelu", "silu", "relu", "none"),
+                                  ((True, True), (False, True), (True, True), (True, False))):
+        out, oi = filled(ctx, (m, n), np.float32)
+        pre, pi = filled(ctx, (m, n), np.float32, by=1)
+        ctx.gemm_bias_act_residual(ctx.upload(A.T if ta else A), ctx.upload(B.T if tb else B), ta, tb, bias=dbias if use[0] else None, act=act,
+                                   residual=dres if use[1] else None, pre=pre, out=out)
+        y, p, by, bp = ref.linear_fwd(A, B, bias if use[0] else None, act, res if use[1] else None)
+        within(out.numpy(), y, by, (ta, tb, act))
+        within(pre.numpy(), p, bp, (ta, tb, act, "pre"))
+        assert oi() and pi()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -505,6 +529,9 @@ def test_refusals(ctx):
     refused("overlaps", ctx.clip_grad_norm, [lo, hi], 1.0)
     refused("overlaps", ctx.clip_grad_norm, [a, b], 1.0, outs=[e(8, 8), a])
     refused("overlaps", ctx.clip_grad_norm, [a, a], 1.0)
+    refused("overlaps", ctx.grad_norm, [a], norm=a.reshape(64).rows(5, 6))
+    refused("overlaps", ctx.clip_grad_norm, [a], 1.0, norm=a.reshape(64).rows(63, 64))
+    refused("overlaps", ctx.embedding_fwd, a, ids, out=_view(ctx, ids.ptr, (8, 8)))
     refused("negative", ctx.clip_grad_norm, [a], -1.0)
     refused("negative", ctx.clip_grad_norm, [a], float("nan"))
     refused("in a call of", ctx.clip_grad_norm, [a, ctx.fill((8,), 1.0, np.float64)], 1.0)
