@@ -568,11 +568,12 @@ int embedding_bwd(fx_ctx* c, const T* g, const int64_t* ids, T* dW, i64 n, i64 v
     a.tpp_log = 0;
     int passes = 1;
     while (passes < 4 && (vocab >> (BITS * passes)) != 0) ++passes;  // the largest key is vocab itself
-    // the one-launch sort while its blocks are few and what they read together, 8 bytes per token each, stays below 128 MB.  Whole call,
-    // rows of 8 floats, against the tiled passes (us): 16000 tokens of 30000 ids 24.6 / 42.4, of 260000 44 / 60, 32000 of 130000 40 / 62,
-    // 4000 of a million 64 / 73, 300 of 200000 16.5 / 39, 100 of four million 107 / 104.
+    // The one-launch sort while its blocks are few, what they read together (8 bytes per token each) stays below 128 MB, and a block has
+    // no more than a few rounds of tokens to place.  Whole call against the tiled passes (us), rows of 8 floats: 16000 tokens of 30000 ids
+    // 24.6 / 42.4, of 260000 44 / 60, 32000 of 130000 40 / 62, 4000 of a million 64 / 73, 100 of four million 107 / 104; rows of 64 floats:
+    // 32768 tokens of 1000 ids 46 / 49, of 500 58 / 49, 16384 of 500 35 / 40, 8192 of 200 29 / 25, 4096 of 200 19 / 23.
     const i64 ranges = vocab / BINS + 1;
-    const bool small = n <= RANGE_MAX && ranges <= 8192 && n * ranges <= (1ll << 24);
+    const bool small = n <= RANGE_MAX && ranges <= 8192 && n * ranges <= (1ll << 24) && n <= (passes == 1 ? 4096 : 8192 * ranges);
     const i64 tiles = fx::ceil_div(n, (i64)TILE), entries = tiles * BINS;
     // scratch: [keys][pos] once or twice, the table of counts, the partial rows
     const i64 nkeys = fx::ceil_div(n, (i64)64) * 64, lists = small ? 2 : 4;
