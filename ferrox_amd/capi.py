@@ -680,8 +680,14 @@ class Context:
             if a is not None and (a.shape != tuple(want) or a.dtype != dtype):
                 raise FerroxHipError(1, f"{what}: {name} is {a.shape} {a.dtype}, not {tuple(want)} {dtype}")
 
+    @staticmethod
+    def _ids(what, ids):
+        if ids.dtype != np.int64:
+            raise FerroxHipError(1, f"{what}: ids are {ids.dtype}, not int64")
+
     def embedding_fwd(self, w, ids, scale=1.0, out=None):
         """out[..., :] = scale * w[ids[...], :]; zeros where an id lies outside the table."""
+        self._ids("embedding_fwd", ids)
         vocab, dim = w.shape
         shape = tuple(ids.shape) + (dim,)
         n = math.prod(ids.shape)
@@ -693,6 +699,7 @@ class Context:
 
     def embedding_bwd(self, g, ids, vocab, scale=1.0, out=None):
         """The dense gradient [vocab, dim] of the table from g, the gradient of embedding_fwd's output."""
+        self._ids("embedding_bwd", ids)
         dim = g.shape[-1]
         n = math.prod(ids.shape)
         self._same("embedding_bwd", tuple(ids.shape) + (dim,), g.dtype, g=g)
@@ -845,10 +852,10 @@ class Context:
 
 
 class _RawI64:
-    """int64 device buffer (argmax indices); carved from the f64 pool since both are 8-byte elements."""
+    """int64 device buffer (argmax indices, token ids); carved from the f64 pool since both are 8-byte elements."""
 
     def __init__(self, ctx, n):
-        self._a = ctx.empty((n,), np.float64)
+        self._a, self.shape, self.dtype = ctx.empty((n,), np.float64), (n,), np.dtype(np.int64)
         self.ptr, self.n, self.ctx = self._a.ptr, n, ctx
 
     def numpy(self):

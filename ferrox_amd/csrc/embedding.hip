@@ -538,7 +538,8 @@ int add_and_join(fx_ctx* c, const T* g, const uint32_t* keys, const uint32_t* po
     while (a.tpp_log < 8 && ((i64)V << a.tpp_log) < a.D) ++a.tpp_log;
     const i64 cols = fx::ceil_div(a.D, (i64)V << a.tpp_log), add_blocks = fx::ceil_div((i64)a.pieces, (i64)(256 >> a.tpp_log));
     const i64 blocks = add_blocks + fx::ceil_div(a.vocab, (i64)ZROWS);
-    FX_REQUIRE(blocks <= 0x7fffffff && cols <= 65535 && fx::ceil_div(a.D, (i64)64 * V) <= 65535, "fx_embedding_bwd: too many elements");
+    // a launch has fewer than 2^32 threads: 256 for 64 ids
+    FX_REQUIRE(blocks < (1 << 24) && cols <= 65535 && fx::ceil_div(a.D, (i64)64 * V) <= 65535, "fx_embedding_bwd: too many rows or columns");
     a.add_blocks = (unsigned)add_blocks;
     FX_LAUNCH(dim3((unsigned)blocks, (unsigned)cols), dim3(256), 0, c->stream, (g, keys, pos, dW, edge, scale, a), embedding_add_kernel<T, V>);
     FX_LAUNCH_CHECK();

@@ -251,11 +251,11 @@ int gemm_bias_act_residual(fx_ctx* c, int ta, int tb, i64 M, i64 N, i64 K, const
         if (int rc = launch_zero<T>(c, C, n)) return rc;
         return ex.any() ? gep::launch_pass<T>(c, C, n, N, ex) : FX_OK;
     }
-    if (grows::eligible(ta != 0, tb != 0, M, K)) {
+    if (grows::eligible(ta != 0, tb != 0, M, N, K)) {
         std::lock_guard<std::mutex> lk(c->launch_mutex);
         return grows::run<T>(c, M, N, K, A, B, C, ex);
     }
-    // what fx_gemm_bias_act does already goes its way, same kernels and bits
+    // of the rest, what fx_gemm_bias_act does already goes its way, same kernels and bits
     if (bias && !residual && !pre && act <= fxact::RELU) return gemm<T>(c, ta, tb, M, N, K, A, B, C, bias, act);
     return gemm<T>(c, ta, tb, M, N, K, A, B, C, nullptr, 0, nullptr, nullptr, ex);
 }

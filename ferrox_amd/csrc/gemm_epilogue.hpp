@@ -65,13 +65,10 @@ template <typename T> inline int launch_sum(fx_ctx* c, const T* part, T* out, i6
 // The epilogue as a pass of its own over the stored product.
 template <typename T>
 __global__ __launch_bounds__(256) void pass_kernel(T* C, i64 n, i64 N, const Epilogue<T> ep) {
-    const i64 i = (i64)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    C[i] = ep.finish(C[i], i, ep.bias ? ep.bias[i % N] : T(0));
+    for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < n; i += (i64)gridDim.x * 256) C[i] = ep.finish(C[i], i, ep.bias ? ep.bias[i % N] : T(0));
 }
 template <typename T> inline int launch_pass(fx_ctx* c, T* C, i64 n, i64 N, const Epilogue<T>& ep) {
-    const i64 blocks = fx::ceil_div(n, (i64)256);
-    FX_REQUIRE(blocks <= 0x7fffffff, "matrix product epilogue: too many elements");
+    const i64 blocks = std::min<i64>(fx::ceil_div(n, (i64)256), 1 << 23);  // a launch has fewer than 2^32 threads
     FX_LAUNCH(dim3((unsigned)blocks), dim3(256), 0, c->stream, (C, n, N, ep), pass_kernel<T>);
     FX_LAUNCH_CHECK();
     return FX_OK;

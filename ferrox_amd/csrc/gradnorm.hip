@@ -13,6 +13,8 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <new>
+#include <vector>
 
 #include "vecio.hpp"
 
@@ -162,7 +164,12 @@ template <typename T>
 int check_overlaps(int count, const T* const* g, T* const* out, const int64_t* n, const T* norm, const char* what) {
     struct Span { uintptr_t lo, hi; int k; bool out; };
     std::vector<Span> spans;
-    spans.reserve(2 * (size_t)count + 1);
+    try {
+        spans.reserve(2 * (size_t)count + 1);
+    } catch (const std::bad_alloc&) {
+        fx::set_error("%s: no host memory for %d tensors", what, count);
+        return FX_ERR_OOM;
+    }
     for (int k = 0; k < count; ++k) {
         if (n[k] == 0) continue;
         const uintptr_t bytes = (uintptr_t)n[k] * sizeof(T);

@@ -275,12 +275,13 @@ template <int L, typename F> int with_cut(i64 steps, F&& f) {
 
 // Sizes, and for a chain of pieces the board in the library's scratch, cleared.
 template <typename T>
-int launch_pieces(fx_ctx* c, Shape& s, Board<T>& board, unsigned*& tickets, i64 B, i64 steps, i64 D, i64 piece, bool chain) {
+int launch_pieces(fx_ctx* c, Shape& s, Board<T>& board, unsigned*& tickets, i64 B, i64 steps, i64 D, i64 piece, int waves, bool chain) {
     s.chains = B * D;
     s.T = steps;
     s.D = D;
     const i64 tiles = fx::ceil_div(s.chains, (i64)64), pieces = fx::ceil_div(steps, piece);
-    FX_REQUIRE(tiles <= 0x7fffffff && tiles * pieces <= 0x7fffffff, "gated recurrence: too many chains and steps");
+    // a launch has fewer than 2^32 threads
+    FX_REQUIRE(tiles <= 0x7fffffff && tiles * pieces < (1ll << 32) / (64 * waves), "gated recurrence: too many chains and steps");
     s.tiles = (unsigned)tiles;
     s.pieces = (unsigned)pieces;
     board = {nullptr, nullptr, s.chains, s.chains * pieces};
@@ -321,7 +322,7 @@ int recurrence_fwd(fx_ctx* c, const T* z, const T* x, const T* h0, T* h, i64 B, 
         Shape s;
         Board<T> board;
         unsigned* tickets;
-        if (int rc = launch_pieces<T>(c, s, board, tickets, B, steps, D, W * L, CHAIN)) return rc;
+        if (int rc = launch_pieces<T>(c, s, board, tickets, B, steps, D, W * L, W, CHAIN)) return rc;
         FX_LAUNCH(dim3(s.tiles * s.pieces), dim3(64 * W), 0, c->stream, (z, x, h0, h, s, board, tickets), recurrence_fwd_kernel<T, W, L, CHAIN>);
         FX_LAUNCH_CHECK();
         return FX_OK;
@@ -350,7 +351,7 @@ int recurrence_bwd(fx_ctx* c, const T* dh, const T* z, const T* x, const T* h, c
         Shape s;
         Board<T> board;
         unsigned* tickets;
-        if (int rc = launch_pieces<T>(c, s, board, tickets, B, steps, D, W * L, CHAIN)) return rc;
+        if (int rc = launch_pieces<T>(c, s, board, tickets, B, steps, D, W * L, W, CHAIN)) return rc;
         FX_LAUNCH(dim3(s.tiles * s.pieces), dim3(64 * W), 0, c->stream, (dh, z, x, h, h0, dnext, dz, dx, dh0, s, board, tickets),
                   recurrence_bwd_kernel<T, W, L, CHAIN>);
         FX_LAUNCH_CHECK();

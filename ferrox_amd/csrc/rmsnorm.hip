@@ -4,7 +4,8 @@
 // Both are bound by memory: 2 reads and 2 writes of [rows, D] forward, 3 reads and 1 write backward.  A row stays in registers
 // between its one read and its one write: up to 16 elements per thread, one wave per row up to 1024 elements, a block of 256 up to
 // 4096 and of 1024 up to 16384; longer rows are read twice.  All accesses are 16-byte vectors that start at any element (a row of an
-// odd length moves the next one off the 16-byte grid); only the last, incomplete vector of a row goes element by element.  Sums are held in the tensors' own type (f32 or f64): a thread adds at most 16 terms before the tree of its block.
+// odd length moves the next one off the 16-byte grid); only the last, incomplete vector of a row goes element by element.  Sums are held in the
+// tensors' own type (f32 or f64): a thread adds at most 16 terms before the tree of its block.
 // The weight gradient is added up in registers over the rows that a block takes (thread t owns the same columns in every row), one
 // partial row per block, and the partial rows are added by a second launch in a fixed order: no atomics.
 #include <mutex>
@@ -87,12 +88,16 @@ __global__ __launch_bounds__(1024) void rmsnorm_fwd_long_kernel(const T* x, cons
 template <typename T, int V, int NT, int E>
 int launch_fwd(fx_ctx* c, const T* x, const T* res, const T* w, T eps, T* h, T* y, T* rstd, i64 rows, i64 D) {
     constexpr int BT = block_of(NT);
-    const i64 blocks = fx::ceil_div(rows, (i64)(BT / NT));
-    FX_REQUIRE(blocks <= 0x7fffffff, "fx_rmsnorm_fwd: too many rows");
-    const dim3 grid((unsigned)blocks), blk(BT);
-    if (res) FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, eps, h, y, rstd, rows, (int)D), rmsnorm_fwd_kernel<T, V, NT, E, true>);
-    else FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, eps, h, y, rstd, rows, (int)D), rmsnorm_fwd_kernel<T, V, NT, E, false>);
-    FX_LAUNCH_CHECK();
+    constexpr i64 MOST = (1ll << 22) * (BT / NT);  // rows of one launch, which has fewer than 2^32 threads
+    const dim3 blk(BT);
+    for (i64 r = 0; r < rows; r += MOST) {
+        const i64 n = std::min(rows - r, MOST), at = r * D;
+        const dim3 grid((unsigned)fx::ceil_div(n, (i64)(BT / NT)));
+        T* const rs = rstd ? rstd + r : nullptr;
+        if (res) FX_LAUNCH(grid, blk, 0, c->stream, (x + at, res + at, w, eps, h + at, y + at, rs, n, (int)D), rmsnorm_fwd_kernel<T, V, NT, E, true>);
+        else FX_LAUNCH(grid, blk, 0, c->stream, (x + at, nullptr, w, eps, nullptr, y + at, rs, n, (int)D), rmsnorm_fwd_kernel<T, V, NT, E, false>);
+        FX_LAUNCH_CHECK();
+    }
     return FX_OK;
 }
 template <typename T, int V>

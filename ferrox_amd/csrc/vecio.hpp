@@ -28,25 +28,26 @@ template <int V, typename T> __device__ __forceinline__ void store_stream(T* p, 
     __builtin_nontemporal_store(q, reinterpret_cast<Vec<T, V>*>(p));
 }
 
-// The vector at column j of a row that ends at D: whole, or what is left of the row (the rest zero / not stored).
+// The vector at column j < D of a row that ends at D: whole, or what is left of the row (the rest zero / not stored).  Compared by
+// differences: j + V may pass 2^31.
 template <int V, typename T> __device__ __forceinline__ void load_part(const T* row, int j, int D, T (&v)[V]) {
-    if (j + V <= D) {
+    if (V <= D - j) {
         load<V>(row + j, v);
     } else {
 #pragma unroll
         for (int u = 0; u < V; ++u) {
             v[u] = T(0);
-            if (j + u < D) v[u] = row[j + u];
+            if (u < D - j) v[u] = row[(i64)j + u];
         }
     }
 }
 template <int V, typename T> __device__ __forceinline__ void store_part(T* row, int j, int D, const T (&v)[V]) {
-    if (j + V <= D) {
+    if (V <= D - j) {
         store<V>(row + j, v);
     } else {
 #pragma unroll
         for (int u = 0; u < V; ++u)
-            if (j + u < D) row[j + u] = v[u];
+            if (u < D - j) row[(i64)j + u] = v[u];
     }
 }
 

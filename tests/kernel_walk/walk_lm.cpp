@@ -131,6 +131,19 @@ template <typename T> void walk_case(fx_ctx* c, i64 rows, i64 out, i64, int shif
     T *W = b[4].get<T>(out, 0), *X = b[5].get<T>(rows, 0), *dX = b[6].get<T>(rows, 0), *dW = b[7].get<T>(out, 0);
     for (int act = 0; act < 4; ++act) check(Act<T>::bwd(c, rows, 1, out, dy, W, X, pre, act, dpre, dX, dW, act & 1 ? db : nullptr), "fx_linear_act_bwd");
     check(Act<T>::bwd(c, rows, 1, out, dy, W, X, pre, 2, dpre, dX, dW, db), "fx_linear_act_bwd");
+    // the last vectors of a row of almost 2^31 elements, of which only the end is there
+    constexpr int V = 16 / (int)sizeof(T), D = 0x7fffffff, LAST = D / V * V;
+    Buf end;
+    T* const tail = end.get<T>(D - LAST + V, 0);  // elements LAST - V .. D - 1
+    T* const row = tail - (LAST - V);
+    T v[V];
+    for (int u = 0; u < D - LAST + V; ++u) tail[u] = T(u + 1);
+    for (int j : {LAST - V, LAST}) {
+        vio::load_part<V>(row, j, D, v);
+        for (int u = 0; u < V; ++u)
+            if (v[u] != (u < D - j ? T(j - (LAST - V) + u + 1) : T(0))) check(FX_ERR_INVALID, "load_part");
+        vio::store_part<V>(row, j, D, v);
+    }
 }
 #endif
 }  // namespace

@@ -482,6 +482,45 @@ def test_clip_extremes(ctx, dtype):
         assert np.array_equal(a.numpy(), host, equal_nan=True) and (b.numpy() == 2.0).all()
 
 
+# ---- sizes past 2^32 threads of one launch, rows of nearly 2^31 ----------------------------------------------------------------------------------
+def test_rmsnorm_of_many_short_rows(ctx):
+    rows = (1 << 26) + 5
+    x, w = ctx.uniform((rows, 1), 3, -2.0, 2.0), ctx.fill((1,), 0.5)
+    h, y, rstd = ctx.rmsnorm_fwd(x, w, 1e-6, res=x)
+    x, h, y, rstd = (a.numpy().ravel() for a in (x, h, y, rstd))
+    assert np.array_equal(h, x + x)
+    h = h.astype(np.float64)
+    r = 1.0 / np.sqrt(h * h + 1e-6)
+    # the square, the addition and eps each at most u (the root halves them), root, reciprocal: 3.5 u, with room for the division by the row's
+    # length; then two products
+    assert (np.abs(rstd - r) <= 6 * ref.u(np.float32) * r).all()
+    assert (np.abs(y - h * r * 0.5) <= 8 * ref.u(np.float32) * np.abs(h * r * 0.5)).all()
+
+
+def test_one_row_times_many_columns(ctx):
+    n = (1 << 26) + 5
+    a, b, bias = ctx.fill((1, 2), 3.0), ctx.uniform((n, 2), 4, -1.0, 1.0), ctx.uniform((n,), 5, -1.0, 1.0)
+    got = ctx.gemm_bias_act_residual(a, b, tb=True, bias=bias, act="relu", residual=bias.reshape(1, n)).numpy()[0].astype(np.float64)
+    b, bias = b.numpy().astype(np.float64), bias.numpy().astype(np.float64)
+    pre = 3.0 * b[:, 0] + 3.0 * b[:, 1] + bias
+    size = 3.0 * np.abs(b).sum(1) + np.abs(bias)
+    # two products, two additions (the largest chain: four roundings of a term), then the residual's addition
+    assert (np.abs(got - (np.maximum(pre, 0) + bias)) <= 6 * ref.u(np.float32) * (size + np.abs(bias))).all()
+
+
+def test_embedding_of_indices_found_on_the_device(ctx):
+    """The arg-max of a product's rows as the next token ids, without a copy to the host; ids of another type are refused."""
+    from ferrox_amd.capi import FerroxHipError
+    rng = np.random.default_rng(5)
+    logits, w = rng.standard_normal((6, 50)).astype(np.float32), rng.standard_normal((50, 8)).astype(np.float32)
+    best = ctx.upload_ids(np.full(6, -1))
+    ctx.reduce_max_noalloc(ctx.upload(logits), 1, ctx.empty((6,)), best)
+    assert np.array_equal(ctx.embedding_fwd(ctx.upload(w), best).numpy(), w[logits.argmax(1)])
+    for call in (lambda: ctx.embedding_fwd(ctx.upload(w), ctx.fill((6,), 1.0)), lambda: ctx.embedding_bwd(ctx.upload(w[:6]), ctx.fill((6,), 1.0), 50)):
+        with pytest.raises(FerroxHipError, match="int64"):
+            call()
+
+
 # ---- refusals: the host's checks, before any launch ------------------------------------------------------------------------------------------
 def test_refusals(ctx):
     from ferrox_amd.capi import FerroxHipError, lib
