@@ -328,13 +328,22 @@ __global__ __launch_bounds__(NT, 2) void gemm_lds_kernel(const Params p) {
 // Bound by the matrix pipe.  Measured (f32, NN / NT / TN / TT, TFLOP/s; in brackets one 64-deep stage per block, computing and staging in
 // turns, as before): 4096 x 1024 x 4096 131 / 134 / 134 / 138 (117 / 123 / 125 / 121), 4096 x 4096 x 1024 132 / 133 / 133 / 134
 // (124 / 125 / 127 / 126), 2048^3 128 / 134 / 131 / 134 (116 / 120 / 122 / 119); 4096^3 138 to 140 of 157.
+// A . B^T in 128 x 64 tiles: B's rows without padding, their eight 16-byte groups permuted by the row (group q of row r lies at
+// q ^ (r / 2 % 8): 16 rows of a read cover all banks as well), so that three blocks fit on a CU as in the other forms; with the padding
+// two did, and products of several rounds of blocks lost by it (3000 x 3000 x 4096 735 us, so 622; 5000 x 5000 x 128 73.6, so 68.2).
 constexpr int KP = 32, PP = KP + 4;
-template <int TN, bool TA, bool TB> constexpr int pipe_stage_floats() { return (TA ? KP * 128 : 128 * PP) + (TB ? 32 * TN * PP : KP * 32 * TN); }
+template <int TN, bool TA, bool TB> constexpr bool pipe_permuted() { return TN == 2 && !TA && TB; }
+template <int TN, bool TA, bool TB> constexpr int pipe_b_pitch() { return TB ? (pipe_permuted<TN, TA, TB>() ? KP : PP) : 32 * TN; }
+template <int TN, bool TA, bool TB> constexpr int pipe_stage_floats() {
+    return (TA ? KP * 128 : 128 * PP) + (TB ? 32 * TN : KP) * pipe_b_pitch<TN, TA, TB>();
+}
 template <int TN, bool TA, bool TB, int EP, bool KT = false>
 __global__ __launch_bounds__(NT, 2) void gemm_pipe_kernel(const Params p) {
     static_assert(!KT || (!TA && TB), "the K tail is handled for k-contiguous operands");
     constexpr int BM = 128, BN = 32 * TN;
     constexpr int ASZ = TA ? KP * BM : BM * PP, STAGE = pipe_stage_floats<TN, TA, TB>();
+    constexpr bool PERM = pipe_permuted<TN, TA, TB>();
+    constexpr int PB = pipe_b_pitch<TN, TA, TB>();
     constexpr int NA = BM * KP / 4 / NT, NB = BN * KP / 4 / NT;  // float4 per thread per stage
     FX_DYNAMIC_SMEM(float, smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
@@ -398,7 +407,12 @@ __global__ __launch_bounds__(NT, 2) void gemm_pipe_kernel(const Params p) {
         const bool is_a = u < NA, kc = is_a ? !TA : TB;  // k-contiguous: even k, then odd k
         const int R = is_a ? BM : BN, Q = R / 4, w = is_a ? u : u - NA;
         float* const d = smem + buf * STAGE + (is_a ? 0 : ASZ);
-        if (kc) {
+        if (kc && !is_a && PERM) {
+            const int row = (tid >> 3) + 32 * w, q = ((tid & 7) >> 1) ^ (row >> 1 & 7);
+            float* const r = d + row * PB + 2 * (tid & 1);
+            *reinterpret_cast<float2*>(r + 4 * q) = make_float2(x.x, x.z);
+            *reinterpret_cast<float2*>(r + 4 * (q ^ 4)) = make_float2(x.y, x.w);
+        } else if (kc) {
             float* const r = d + ((tid >> 3) + 32 * w) * PP + 2 * (tid & 7);
             *reinterpret_cast<float2*>(r) = make_float2(x.x, x.z);
             *reinterpret_cast<float2*>(r + KP / 2) = make_float2(x.y, x.w);
@@ -409,7 +423,10 @@ __global__ __launch_bounds__(NT, 2) void gemm_pipe_kernel(const Params p) {
 
     // operands of four MFMA steps (group g: steps 4 g .. 4 g + 3)
     const float* const ar = TA ? smem + half * BM + wave * 32 + l32 : smem + (wave * 32 + l32) * PP + half * (KP / 2);
-    const float* const br = TB ? smem + ASZ + l32 * PP + half * (KP / 2) : smem + ASZ + half * BN + l32;
+    const float* const br = TB ? smem + ASZ + l32 * PB + (PERM ? 0 : half * (KP / 2)) : smem + ASZ + half * BN + l32;
+    int group[4];  // PERM: where groups 0 .. 3 of this lane's half lie in its rows (l32 and l32 + 32 are permuted alike)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) group[g] = PERM ? 4 * ((4 * half + g) ^ (l32 >> 1 & 7)) : 4 * g;
     auto read = [&](float (&a)[4], float (&b)[TN][4], int buf, int g) __attribute__((always_inline)) {
         const float* const x = ar + buf * STAGE;
         const float* const y = br + buf * STAGE;
@@ -423,7 +440,7 @@ __global__ __launch_bounds__(NT, 2) void gemm_pipe_kernel(const Params p) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             if (TB) {
-                const float4 v = *reinterpret_cast<const float4*>(y + j * 32 * PP + 4 * g);
+                const float4 v = *reinterpret_cast<const float4*>(y + j * 32 * PB + group[g]);
                 b[j][0] = v.x; b[j][1] = v.y; b[j][2] = v.z; b[j][3] = v.w;
             } else {
 #pragma unroll
@@ -547,6 +564,7 @@ inline Plan make_plan(int num_cus, bool ta, bool tb, i64 M, i64 N, i64 K, i64 ld
 
 template <int TN, bool TA, bool TB, int EP, bool KT> inline int launch_pipe_ep(fx_ctx* c, const Params& p, dim3 grid, dim3 blk) {
     constexpr size_t lds = 2 * sizeof(float) * pipe_stage_floats<TN, TA, TB>();
+    static_assert(TN != 2 || 3 * lds <= 160 * 1024, "three blocks of the 128 x 64 tiles share a CU's LDS");
     static const hipError_t attr = hipFuncSetAttribute((const void*)gemm_pipe_kernel<TN, TA, TB, EP, KT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     FX_HIP_CHECK(attr);
     FX_LAUNCH(grid, blk, lds, c->stream, (p), gemm_pipe_kernel<TN, TA, TB, EP, KT>);
