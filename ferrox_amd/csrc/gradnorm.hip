@@ -9,7 +9,13 @@
 // The tensor table travels in the kernel's arguments, which lie in host memory: every block copies it to LDS once, all entries in
 // flight together, and finds a chunk's tensor by a ballot.
 // Squares are added in f64 whatever the tensors' type: f32 gradients neither overflow nor lose small terms, and the extra work is
-// hidden behind the loads.  Everything is summed in a fixed order, no atomics.
+// hidden behind the loads.  Squares of f64 gradients can leave the range of f64 at either end: a thread adds a chunk's squares as they
+// are and, where that sum is no good (it overflowed, or is so small that terms may have vanished), adds them again in three sums, of the
+// large elements times 2^-600, of the small ones times 2^600 and of the rest.  A block whose two outer sums hold anything stores them
+// and marks its partial by a negative sign; they are read only then (113 million f64 elements clipped: 502 us, with one sum alone 505).
+// Everything is summed in a fixed order, no atomics.
+// The norm is kept as root * 2^e until the factor max / norm is formed, which therefore has full precision wherever the norm lies.
+// Elements that are infinite or NaN give such a norm, and nothing is scaled.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -23,6 +29,8 @@ using namespace vio;
 
 constexpr int NT = 256, CHUNK = 4096, TABLE = 96;  // elements of a chunk; tensors of one launch (the table travels in the arguments)
 constexpr int MAX_PARTIALS = 2048;
+// Elements above LARGE or below SMALL go to the outer sums: squares of the ones between lie in 2^-1022 .. 2^972, and 2^50 of them fit.
+constexpr double LARGE = 0x1p486, SMALL = 0x1p-511, UP = 0x1p600, DOWN = 0x1p-600;
 
 template <typename T> struct Tensors {
     const T* g[TABLE];
@@ -60,13 +68,26 @@ __device__ __forceinline__ int tensor_of(const Starts& s, unsigned chunk) {  // 
     return __popcll(__ballot(s.a <= chunk)) + __popcll(__ballot(s.b <= chunk)) - 1;
 }
 
+// Sums of squares: of the elements between SMALL and LARGE, of the larger ones times DOWN, of the smaller ones times UP.
+struct Squares {
+    double mid = 0., large = 0., small = 0.;
+    __device__ __forceinline__ void add(double v) {
+        const double a = fabs(v);
+        if (!(a <= LARGE)) large = fma(v * DOWN, v * DOWN, large);  // NaN too
+        else if (a < SMALL) small = fma(v * UP, v * UP, small);
+        else mid = fma(v, v, mid);
+    }
+};
+
+// part: 3 planes of `plane` partial sums (f32: the first one only)
 template <typename T>
-__global__ __launch_bounds__(NT) void sum_squares_kernel(const Tensors<T> tt, double* __restrict__ part) {
+__global__ __launch_bounds__(NT) void sum_squares_kernel(const Tensors<T> tt, double* __restrict__ part, i64 plane) {
     constexpr int V = 16 / (int)sizeof(T), PER = CHUNK / NT / V;
-    __shared__ double sm[NT / 64 + 1];
+    constexpr bool WIDE = sizeof(T) == 8;
+    __shared__ double sm[3][NT / 64 + 1];
     __shared__ Table<T> tab;
     const Starts starts = stage_table(tt, tab);
-    double s = 0.;
+    Squares s;
     const unsigned chunks = tt.first[tt.count];
     for (unsigned q = blockIdx.x; q < chunks; q += gridDim.x) {
         const int t = tensor_of(starts, q);
@@ -77,42 +98,113 @@ __global__ __launch_bounds__(NT) void sum_squares_kernel(const Tensors<T> tt, do
             T v[PER][V];
 #pragma unroll
             for (int k = 0; k < PER; ++k) load<V>(g + (k * NT + threadIdx.x) * V, v[k]);
+            double sum = s.mid;
 #pragma unroll
             for (int k = 0; k < PER; ++k)
 #pragma unroll
-                for (int u = 0; u < V; ++u) s = fma((double)v[k][u], (double)v[k][u], s);
+                for (int u = 0; u < V; ++u) sum = fma((double)v[k][u], (double)v[k][u], sum);
+            // below 2^-900, terms that vanished could count; a sum of zeros comes here too and is added again for nothing
+            if (!WIDE || (sum >= 0x1p-900 && sum <= 0x1p1000)) {
+                s.mid = sum;
+            } else {
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+#pragma unroll
+                    for (int u = 0; u < V; ++u) s.add((double)v[k][u]);
+            }
         } else {
-            for (int j = threadIdx.x; j < left; j += NT) s = fma((double)g[j], (double)g[j], s);
+            for (int j = threadIdx.x; j < left; j += NT) {
+                if constexpr (WIDE) s.add((double)g[j]);
+                else s.mid = fma((double)g[j], (double)g[j], s.mid);
+            }
         }
     }
-    s = block_sum<NT>(s, sm);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    double mid = block_sum<NT>(s.mid, sm[0]);
+    if constexpr (WIDE) {
+        if (__syncthreads_or(!(s.large == 0. && s.small == 0.))) {
+            mid = -mid;  // minus zero as well
+            const double large = block_sum<NT>(s.large, sm[1]), small = block_sum<NT>(s.small, sm[2]);
+            if (threadIdx.x == 0) {
+                part[plane + blockIdx.x] = large;
+                part[2 * plane + blockIdx.x] = small;
+            }
+        }
+    }
+    if (threadIdx.x == 0) part[blockIdx.x] = mid;
 }
 
-// sqrt of the sum of all partials, the same bits in every block
-__device__ __forceinline__ double norm_of(const double* __restrict__ part, int parts, double* sm) {
+struct Norm {  // root * 2^e
+    double root;
+    int e;
+    __device__ __forceinline__ double value() const { return ldexp(root, e); }
+};
+// The norm from all partials, the same bits in every block.
+template <bool WIDE> __device__ __forceinline__ Norm norm_of(const double* __restrict__ part, i64 plane, int parts, double (*sm)[NT / 64 + 1]) {
     double s = 0.;
-    for (int j = threadIdx.x; j < parts; j += NT) s = s + part[j];
-    return sqrt(block_sum<NT>(s, sm));
+    int marked = 0;
+    for (int j = threadIdx.x; j < parts; j += NT) {
+        const double p = part[j];
+        marked |= __double2hiint(p) < 0;
+        s = s + fabs(p);
+    }
+    s = block_sum<NT>(s, sm[0]);
+    if constexpr (WIDE) {
+        if (__syncthreads_or(marked)) {
+            double large = 0., small = 0.;
+            for (int j = threadIdx.x; j < parts; j += NT) {
+                if (__double2hiint(part[j]) >= 0) continue;
+                large = large + part[plane + j];
+                small = small + part[2 * plane + j];
+            }
+            large = block_sum<NT>(large, sm[1]);
+            small = block_sum<NT>(small, sm[2]);
+            if (!(large == 0.)) return {sqrt(large + s * DOWN * DOWN), 600};
+            if (s < 0x1p-400) return {sqrt(s * UP * UP + small), -600};
+        }
+    }
+    return {sqrt(s), 0};
+}
+
+// max_norm / norm as c * 2^e; e is 0 unless the quotient is below the type's normal numbers (or max_norm is subnormal)
+template <typename T> struct Factor {
+    T c;
+    int e;
+    __device__ __forceinline__ T times(T g) const {
+        const T v = g * c;
+        return e ? ldexp(v, e) : v;
+    }
+};
+template <typename T> __device__ __forceinline__ Factor<T> factor_of(const Norm& norm, double max_norm) {
+    constexpr double LEAST = sizeof(T) == 4 ? 0x1p-126 : 0x1p-1022;  // the smallest normal number
+    constexpr int LEAST_E = sizeof(T) == 4 ? -126 : -1022;
+    const double most = ldexp(max_norm, -norm.e);
+    if (!(norm.root > most) || !(norm.root <= 1.7976931348623157e308)) return {T(1), 0};  // nothing to scale, or infinite or NaN
+    if (max_norm == 0.) return {T(0), 0};
+    const double q = most / norm.root;
+    if (most >= 0x1p-1022 && q >= LEAST) return {(T)q, 0};  // rounded once to the tensors' type
+    int em, er;
+    const double c = 0.5 * frexp(max_norm, &em) / frexp(norm.root, &er);  // in 1/4 .. 1
+    const int e = em - er - norm.e + 1;
+    if (e > LEAST_E + 2) return {(T)ldexp(c, e), 0};
+    return {(T)c, e};
 }
 
 template <typename T>
-__global__ __launch_bounds__(NT) void norm_kernel(const double* __restrict__ part, int parts, T* __restrict__ norm) {
-    __shared__ double sm[NT / 64 + 1];
-    const double v = norm_of(part, parts, sm);
-    if (threadIdx.x == 0) norm[0] = (T)v;
+__global__ __launch_bounds__(NT) void norm_kernel(const double* __restrict__ part, i64 plane, int parts, T* __restrict__ norm) {
+    __shared__ double sm[3][NT / 64 + 1];
+    const Norm v = norm_of<sizeof(T) == 8>(part, plane, parts, sm);
+    if (threadIdx.x == 0) norm[0] = (T)v.value();
 }
 
 template <typename T>
-__global__ __launch_bounds__(NT) void scale_kernel(const Tensors<T> tt, const double* __restrict__ part, int parts, double max_norm, T* norm) {
+__global__ __launch_bounds__(NT) void scale_kernel(const Tensors<T> tt, const double* __restrict__ part, i64 plane, int parts, double max_norm, T* norm) {
     constexpr int V = 16 / (int)sizeof(T), PER = CHUNK / NT / V;
-    __shared__ double sm[NT / 64 + 1];
+    __shared__ double sm[3][NT / 64 + 1];
     __shared__ Table<T> tab;
     const Starts starts = stage_table(tt, tab);
-    const double total = norm_of(part, parts, sm);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (T)total;
-    // the factor rounded once to the tensors' type; a norm that is infinite or NaN scales nothing
-    const T coef = total > max_norm && total <= 1.7976931348623157e308 ? (T)(max_norm / total) : T(1);
+    const Norm total = norm_of<sizeof(T) == 8>(part, plane, parts, sm);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (T)total.value();
+    const Factor<T> factor = factor_of<T>(total, max_norm);
     const unsigned chunks = tt.first[tt.count];
     for (unsigned q0 = blockIdx.x; q0 < chunks; q0 += gridDim.x) {
         const unsigned q = chunks - 1 - q0;
@@ -120,7 +212,7 @@ __global__ __launch_bounds__(NT) void scale_kernel(const Tensors<T> tt, const do
         const i64 at = (i64)(q - tab.first[t]) * CHUNK;
         const T* g = tab.g[t] + at;
         T* o = tab.out[t] + at;
-        if (coef == T(1) && g == o) continue;  // in place and nothing to scale
+        if (factor.c == T(1) && factor.e == 0 && g == o) continue;  // in place and nothing to scale
         const i64 left = tab.n[t] - at;
         if (left >= CHUNK) {
             T v[PER][V];
@@ -129,11 +221,11 @@ __global__ __launch_bounds__(NT) void scale_kernel(const Tensors<T> tt, const do
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
 #pragma unroll
-                for (int u = 0; u < V; ++u) v[k][u] = v[k][u] * coef;
+                for (int u = 0; u < V; ++u) v[k][u] = factor.times(v[k][u]);
                 store<V>(o + (k * NT + threadIdx.x) * V, v[k]);
             }
         } else {
-            for (int j = threadIdx.x; j < left; j += NT) o[j] = g[j] * coef;
+            for (int j = threadIdx.x; j < left; j += NT) o[j] = factor.times(g[j]);
         }
     }
 }
@@ -210,20 +302,21 @@ int grad_norm(fx_ctx* c, int count, const T* const* g, T* const* out, const int6
         if (tt.count) ++launches;
     }
     const i64 per_launch = std::max<i64>(1, std::min<i64>(8 * (i64)c->num_cus, MAX_PARTIALS / std::max(1, launches)));
-    double* part = (double*)c->get_scratch(std::max<i64>(1, per_launch * launches) * (i64)sizeof(double));
+    const i64 plane = std::max<i64>(1, per_launch * launches);
+    double* part = (double*)c->get_scratch((sizeof(T) == 8 ? 3 : 1) * plane * (i64)sizeof(double));
     if (!part) return FX_ERR_OOM;
     i64 parts = 0;
     for (int k = 0; k < count;) {
         k = fill_table<T>(tt, k, count, g, out, n);
         if (!tt.count) continue;
         const i64 blocks = std::min<i64>(per_launch, tt.first[tt.count]);
-        FX_LAUNCH(dim3((unsigned)blocks), dim3(NT), 0, c->stream, (tt, part + parts), sum_squares_kernel<T>);
+        FX_LAUNCH(dim3((unsigned)blocks), dim3(NT), 0, c->stream, (tt, part + parts, plane), sum_squares_kernel<T>);
         FX_LAUNCH_CHECK();
         parts += blocks;
     }
     FX_REQUIRE(parts <= 0x7fffffff, "%s: too many tensors", what);
     if (!out || parts == 0) {
-        FX_LAUNCH(dim3(1), dim3(NT), 0, c->stream, (part, (int)parts, norm), norm_kernel<T>);
+        FX_LAUNCH(dim3(1), dim3(NT), 0, c->stream, (part, plane, (int)parts, norm), norm_kernel<T>);
         FX_LAUNCH_CHECK();
         return FX_OK;
     }
@@ -232,7 +325,7 @@ int grad_norm(fx_ctx* c, int count, const T* const* g, T* const* out, const int6
         k = fill_table<T>(tt, k, count, g, out, n);
         if (!tt.count) continue;
         const i64 blocks = std::min<i64>(8 * (i64)c->num_cus, tt.first[tt.count]);
-        FX_LAUNCH(dim3((unsigned)blocks), dim3(NT), 0, c->stream, (tt, part, (int)parts, max_norm, norm_out), scale_kernel<T>);
+        FX_LAUNCH(dim3((unsigned)blocks), dim3(NT), 0, c->stream, (tt, part, plane, (int)parts, max_norm, norm_out), scale_kernel<T>);
         FX_LAUNCH_CHECK();
         norm_out = nullptr;
     }

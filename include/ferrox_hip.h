@@ -435,8 +435,9 @@ enum fx_scalar_op { FX_ADD_SCALAR = 0, FX_SUB_SCALAR = 1, FX_MUL_SCALAR = 2, FX_
        the same tables (HOST arrays of `count` device pointers / element counts): norm[0] (on the device) = sqrt of the sum\
        of g*g over all tensors; clip: out[k] = g[k] * (norm > max_norm ? max_norm/norm : 1).  out[k] may be g[k] (nothing is\
        written then where nothing is scaled), and shares memory with no other tensor of the call.  Squares are added in\
-       double for both types, in a fixed order.  A norm that is infinite or NaN scales nothing: the caller finds it in \
-       norm[0].  No host synchronisation: the calls may be recorded (fx_graph_*). */                                   \
+       double for both types, in a fixed order; finite gradients of any magnitude are clipped by their norm, also where\
+       norm[0] lies beyond the type and reads infinity.  Where an element is infinite or NaN, so is norm[0], and nothing\
+       is scaled.  No host synchronisation: the calls may be recorded (fx_graph_*). */                                 \
     int fx_grad_norm_multi_##S(fx_ctx* ctx, int count, const T* const* g, const int64_t* n, T* norm);                  \
     int fx_clip_grad_norm_multi_##S(fx_ctx* ctx, int count, const T* const* g, T* const* out, const int64_t* n,        \
                                     double max_norm, T* norm);
