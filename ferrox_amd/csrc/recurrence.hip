@@ -33,12 +33,33 @@ using namespace vio;
 __device__ __forceinline__ float dev_exp(float x) { return expf(x); }
 __device__ __forceinline__ double dev_exp(double x) { return exp(x); }
 
+typedef unsigned long long u64;
+
 // f = sigmoid(z) and k = sigmoid(-z), both to full relative precision, from one exponential of -|z| (never overflows)
 template <typename T> __device__ __forceinline__ void gate(T z, T& f, T& k) {
     const T e = dev_exp(z < T(0) ? z : -z);
     const T big = T(1) / (T(1) + e), small = e * big;
     f = z < T(0) ? small : big;
     k = z < T(0) ? big : small;
+}
+
+// A product of gates that underflows though none of them is 0 is held as minus zero: an infinite state stays infinite under it, and
+// becomes NaN under a product with a gate of 0.  Both products times infinity are NaN, so the maps are folded plainly, and once more by
+// the functions below only where the result is NaN.
+__device__ __forceinline__ bool is_minus_zero(float a) { return __float_as_uint(a) == 0x80000000u; }
+__device__ __forceinline__ bool is_minus_zero(double a) { return (u64)__double_as_longlong(a) == 1ull << 63; }
+// of gates, the smallest of them `least`
+template <typename T> __device__ __forceinline__ T product_of(T A, T least) { return A == T(0) && least > T(0) ? -T(0) : A; }
+// of two products
+template <typename T> __device__ __forceinline__ T times(T a, T b) {
+    const T p = a * b;
+    if (p != T(0)) return p;  // NaN too
+    return (a > T(0) || is_minus_zero(a)) && (b > T(0) || is_minus_zero(b)) ? -T(0) : T(0);
+}
+// the map (A, H) of the state v
+template <typename T> __device__ __forceinline__ T mapped(T A, T H, T v) {
+    const T r = A * v + H;
+    return r != r && is_minus_zero(A) && v - v != T(0) ? v + H : r;
 }
 
 struct Shape {
@@ -50,7 +71,6 @@ struct Shape {
 __device__ __forceinline__ i64 chain_base(const Shape& s, i64 c) { return (c / s.D) * (s.T * s.D) + c % s.D; }
 
 // ---- what pieces hand to each other ---------------------------------------------------------------------------------------------
-typedef unsigned long long u64;
 constexpr u64 EMPTY = ~0ull;
 constexpr unsigned GROUP = 32;
 
@@ -85,6 +105,11 @@ template <> struct Board<float> {
         A = __uint_as_float((uint32_t)v);
         H = __uint_as_float((uint32_t)(v >> 32));
     }
+    __device__ __forceinline__ void peek_map(unsigned piece, i64 c, float& A, float& H) const {
+        const u64 v = get(words + piece * chains + c);
+        A = __uint_as_float((uint32_t)v);
+        H = __uint_as_float((uint32_t)(v >> 32));
+    }
     __device__ __forceinline__ void put_state(unsigned g, i64 c, float v) const { put(states + g * chains + c, (u64)__float_as_uint(plain_nan(v))); }
     __device__ __forceinline__ float get_state(unsigned g, i64 c) const { return __uint_as_float((uint32_t)await(states + g * chains + c)); }
 };
@@ -101,6 +126,10 @@ template <> struct Board<double> {
         A = __longlong_as_double((long long)await(words + piece * chains + c));
         H = __longlong_as_double((long long)await(words + plane + piece * chains + c));
     }
+    __device__ __forceinline__ void peek_map(unsigned piece, i64 c, double& A, double& H) const {
+        A = __longlong_as_double((long long)get(words + piece * chains + c));
+        H = __longlong_as_double((long long)get(words + plane + piece * chains + c));
+    }
     __device__ __forceinline__ void put_state(unsigned g, i64 c, double v) const { put(states + g * chains + c, (u64)__double_as_longlong(plain_nan(v))); }
     __device__ __forceinline__ double get_state(unsigned g, i64 c) const { return __longlong_as_double((long long)await(states + g * chains + c)); }
 };
@@ -116,7 +145,7 @@ __global__ __launch_bounds__(256) void board_clear_kernel(u64* __restrict__ p, i
 // The state in front of this wave's steps.  (A, H): the wave's own map; start: the state in front of piece 0.  All waves call it.
 template <typename T, int W, bool CHAIN>
 __device__ __forceinline__ T state_before(T A, T H, T start, unsigned piece, unsigned pieces, i64 chain, bool live, const Board<T>& board) {
-    __shared__ T mapA[W][64], mapH[W][64];
+    __shared__ T mapA[W][64], mapH[W][64], base[CHAIN ? 64 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if constexpr (W > 1 || CHAIN) {
         mapA[wave][lane] = A;
@@ -125,13 +154,21 @@ __device__ __forceinline__ T state_before(T A, T H, T start, unsigned piece, uns
     }
     T v = start;
     if constexpr (CHAIN) {
-        __shared__ T preA[W][64], preH[W][64], base[64];
+        __shared__ T preA[W][64], preH[W][64];
         if (wave == W - 1 && piece + 1 < pieces) {  // publish first
             T a = mapA[0][lane], h = mapH[0][lane];
 #pragma unroll
             for (int w = 1; w < W; ++w) {
                 h = mapA[w][lane] * h + mapH[w][lane];
                 a = a * mapA[w][lane];
+            }
+            if (a == T(0) || h != h) {
+                a = mapA[0][lane], h = mapH[0][lane];
+#pragma unroll 1
+                for (int w = 1; w < W; ++w) {
+                    h = mapped(mapA[w][lane], mapH[w][lane], h);
+                    a = times(a, mapA[w][lane]);
+                }
             }
             if (live) board.put_map(piece, chain, a, h);
         }
@@ -155,6 +192,19 @@ __device__ __forceinline__ T state_before(T A, T H, T start, unsigned piece, uns
 #pragma unroll
     for (int w = 0; w < W - 1; ++w)
         if (w < wave) v = mapA[w][lane] * v + mapH[w][lane];
+    if (v != v) {  // once more, map by map
+        v = start;
+        if constexpr (CHAIN) {
+            v = base[lane];
+            for (unsigned j = piece / GROUP * GROUP; j < piece; ++j) {  // all published: some wave of this block has waited for each
+                T a, h;
+                board.peek_map(j, chain, a, h);
+                v = mapped(a, h, v);
+            }
+        }
+#pragma unroll 1
+        for (int w = 0; w < wave; ++w) v = mapped(mapA[w][lane], mapH[w][lane], v);
+    }
     return v;
 }
 
@@ -186,7 +236,7 @@ __global__ __launch_bounds__(64 * W) void recurrence_fwd_kernel(const T* __restr
         u[l] = x[at];
     }
     const T start = h0 ? h0[chain] : T(0);
-    T A = T(1), H = T(0);
+    T A = T(1), H = T(0), least = T(1);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         T k;
@@ -195,9 +245,10 @@ __global__ __launch_bounds__(64 * W) void recurrence_fwd_kernel(const T* __restr
         if (ts + l < s.T) {
             H = f[l] * H + u[l];
             A = A * f[l];
+            least = min(least, f[l]);
         }
     }
-    T v = state_before<T, W, CHAIN>(A, H, start, piece, s.pieces, chain, live, board);
+    T v = state_before<T, W, CHAIN>(product_of(A, least), H, start, piece, s.pieces, chain, live, board);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         v = f[l] * v + u[l];
@@ -227,7 +278,7 @@ __global__ __launch_bounds__(64 * W) void recurrence_bwd_kernel(const T* __restr
         e[l] = *(t > 0 ? h + (at - s.D) : h0 ? h0 + chain : x + at);  // in front of step 0: h0, or what the next loop replaces by 0
     }
     const T start = dnext ? dnext[chain] : T(0);
-    T A = T(1), H = T(0);
+    T A = T(1), H = T(0), least = T(1);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         if (qs + l >= s.T - 1 && !h0) e[l] = T(0);
@@ -237,9 +288,10 @@ __global__ __launch_bounds__(64 * W) void recurrence_bwd_kernel(const T* __restr
         if (qs + l < s.T) {
             H = f[l] * (g[l] + H);
             A = A * f[l];
+            least = min(least, f[l]);
         }
     }
-    T v = state_before<T, W, CHAIN>(A, H, start, piece, s.pieces, chain, live, board);
+    T v = state_before<T, W, CHAIN>(product_of(A, least), H, start, piece, s.pieces, chain, live, board);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         if (qs + l < s.T) {

@@ -426,7 +426,8 @@ enum fx_scalar_op { FX_ADD_SCALAR = 0, FX_SUB_SCALAR = 1, FX_MUL_SCALAR = 2, FX_
        h_{-1} = h0 [B, dim] (NULL: 0).  The last step's h is the next segment's h0; steps = 1 is the generating form.  \
        bwd, from dh [B, steps, dim] and dh_next [B, dim], the gradient that arrives at the last state from the next segment\
        (its dh0; NULL: none): dz, dx [B, steps, dim] and dh0 [B, dim] (may be NULL), with h and h0 as in the forward call.\
-       Outputs share memory with nothing else. */                                                                      \
+       An infinite state stays so until a gate is 0 (then it is NaN), at any length.  Outputs share memory with nothing\
+       else. */                                                                                                        \
     int fx_gated_recurrence_fwd_##S(fx_ctx* ctx, const T* z, const T* x, const T* h0, T* h, int64_t B, int64_t steps,  \
                                     int64_t dim);                                                                      \
     int fx_gated_recurrence_bwd_##S(fx_ctx* ctx, const T* dh, const T* z, const T* x, const T* h, const T* h0,         \
