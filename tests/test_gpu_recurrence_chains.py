@@ -1,8 +1,10 @@
-"""What the pieces of a long recurrence hand on to one another: infinite states against the definition step by step."""
+"""What the pieces of a long recurrence hand on to one another: infinite states against the definition step by step, states carried over
+dozens of pieces."""
 import numpy as np
 import pytest
 
 import lm_reference as ref
+import recurrence_chains as rc
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +55,14 @@ def test_infinite_states(ctx, B, T, D, dtype):
     outs = ctx.gated_recurrence_bwd(ctx.upload(dh), ctx.upload(z), ctx.upload(tame), ctx.upload(h), None, ctx.upload(nxt), want_dh0=True)
     for o, w, b, name in zip(outs, back, bounds, ("dz", "dx", "dh0")):
         as_defined(o.numpy(), w, b, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D", rc.SHAPES)
+def test_states_carried_over_many_pieces(ctx, B, T, D, dtype):
+    z, x, h0, dh, nxt = rc.inputs(B, T, D, dtype)
+    up = {name: ctx.upload(a) for name, a in (("z", z), ("x", x), ("h0", h0), ("dh", dh), ("nxt", nxt))}
+    h = ctx.gated_recurrence_fwd(up["z"], up["x"], up["h0"])
+    rc.check_forward(h.numpy().astype(np.float64), z, x, h0)
+    dz, dx, dh0 = ctx.gated_recurrence_bwd(up["dh"], up["z"], up["x"], h, up["h0"], up["nxt"])
+    rc.check_backward(*(a.numpy().astype(np.float64) for a in (dz, dx, dh0)), dh, z, x, h.numpy(), h0, nxt)
