@@ -321,7 +321,9 @@ template <int L, typename F> int with_cut(i64 steps, F&& f) {
     if (steps == 1) return f(Cut<1, 1>(), std::false_type());
     if (steps <= 8) return f(Cut<1, 8>(), std::false_type());
     if (steps <= 32) return f(Cut<4, 8>(), std::false_type());
-    if (steps <= 8 * L) return f(Cut<8, L>(), std::false_type());
+    if constexpr (8 * L > 32) {
+        if (steps <= 8 * L) return f(Cut<8, L>(), std::false_type());
+    }
     return f(Cut<8, L>(), std::true_type());
 }
 
