@@ -516,10 +516,13 @@ int embedding_fwd(fx_ctx* c, const T* W, const int64_t* ids, T* out, i64 n, i64 
     FX_REQUIRE(!fx::overlap(out, n * D, W, vocab * D) && !fx::overlap((const char*)out, n * D * (i64)sizeof(T), (const char*)ids, n * 8),
                "fx_embedding_fwd: the output overlaps an input");
     constexpr int V = 16 / (int)sizeof(T);
-    const i64 nv = fx::ceil_div(D, (i64)V), total = n * nv, blocks = fx::ceil_div(total, (i64)1024);
-    FX_REQUIRE(blocks <= 0x7fffffff, "fx_embedding_fwd: too many elements");
-    FX_LAUNCH(dim3((unsigned)blocks), dim3(256), 0, c->stream, (W, ids, out, total, (unsigned)nv, vocab, (int)D, scale), embedding_fwd_kernel<T, V>);
-    FX_LAUNCH_CHECK();
+    const i64 nv = fx::ceil_div(D, (i64)V), most = 0xffffffll * 1024 / nv;  // tokens of one launch, which has fewer than 2^32 threads
+    for (i64 k = 0; k < n; k += most) {
+        const i64 total = std::min(n - k, most) * nv;
+        FX_LAUNCH(dim3((unsigned)fx::ceil_div(total, (i64)1024)), dim3(256), 0, c->stream,
+                  (W, ids + k, out + k * D, total, (unsigned)nv, vocab, (int)D, scale), embedding_fwd_kernel<T, V>);
+        FX_LAUNCH_CHECK();
+    }
     return FX_OK;
 }
 

@@ -14,13 +14,13 @@ namespace {
 using namespace vio;
 
 // One thread per column vector, rows strided over blockIdx.y: block (x, y) leaves the column sums of rows y, y + gridDim.y, ... in part[y].
-// G row groups of 64 threads share a block; their sums are added in group order.
+// G row groups of 64 threads share a block; their sums are added in group order.  first: where the launch's columns begin.
 constexpr int GROUPS = 4;
 template <typename T, int V, int ACT>
-__global__ __launch_bounds__(64 * GROUPS) void act_bwd_kernel(const T* dy, const T* pre, T* dpre, T* __restrict__ part, i64 rows, i64 cols) {
+__global__ __launch_bounds__(64 * GROUPS) void act_bwd_kernel(const T* dy, const T* pre, T* dpre, T* __restrict__ part, i64 rows, i64 cols, i64 first) {
     __shared__ T sm[GROUPS][64 * V];
     const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
-    const i64 c = ((i64)blockIdx.x * 64 + lane) * V;
+    const i64 c = first + ((i64)blockIdx.x * 64 + lane) * V;
     const bool live = c < cols;
     T s[V];
 #pragma unroll
@@ -64,19 +64,22 @@ __global__ __launch_bounds__(64 * GROUPS) void act_bwd_kernel(const T* dy, const
 template <typename T, int V>
 int launch_act_bwd(fx_ctx* c, int act, const T* dy, const T* pre, T* dpre, T* db, i64 rows, i64 cols) {
     const i64 gx = fx::ceil_div(cols, (i64)64 * V);
-    FX_REQUIRE(gx <= 0x7fffffff, "fx_linear_act_bwd: too many columns");
     const i64 gy = std::min<i64>(fx::ceil_div(rows, (i64)GROUPS), std::max<i64>(1, 8 * (i64)c->num_cus / gx));
     T* part = nullptr;
     if (db) {
         part = gy == 1 ? db : (T*)c->get_scratch(gy * cols * (i64)sizeof(T));
         if (!part) return FX_ERR_OOM;
     }
-    const dim3 grid((unsigned)gx, (unsigned)gy), blk(64 * GROUPS);
-    if (act == fxact::RELU) FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols), act_bwd_kernel<T, V, fxact::RELU>);
-    else if (act == fxact::GELU) FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols), act_bwd_kernel<T, V, fxact::GELU>);
-    else if (act == fxact::SILU) FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols), act_bwd_kernel<T, V, fxact::SILU>);
-    else FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols), act_bwd_kernel<T, V, fxact::NONE>);
-    FX_LAUNCH_CHECK();
+    constexpr i64 MOST = 0xffffffffll / (64 * GROUPS);  // blocks along the columns of one launch, which has fewer than 2^32 threads
+    for (i64 b = 0; b < gx; b += MOST) {
+        const dim3 grid((unsigned)std::min(gx - b, MOST), (unsigned)gy), blk(64 * GROUPS);
+        const i64 first = b * 64 * V;
+        if (act == fxact::RELU) FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols, first), act_bwd_kernel<T, V, fxact::RELU>);
+        else if (act == fxact::GELU) FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols, first), act_bwd_kernel<T, V, fxact::GELU>);
+        else if (act == fxact::SILU) FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols, first), act_bwd_kernel<T, V, fxact::SILU>);
+        else FX_LAUNCH(grid, blk, 0, c->stream, (dy, pre, dpre, part, rows, cols, first), act_bwd_kernel<T, V, fxact::NONE>);
+        FX_LAUNCH_CHECK();
+    }
     return db && gy > 1 ? column_sum<T>(c, part, db, (int)gy, cols) : FX_OK;
 }
 

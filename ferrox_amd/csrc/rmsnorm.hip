@@ -63,6 +63,8 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_fwd_kernel(const T* x, c
     }
 }
 
+constexpr i64 MOST_LONG = 0xffffffffll / 1024;  // rows of one launch of the long-row kernels
+
 // Rows longer than a block's registers: the second pass reads the row again (the sum with the residual from h, where this thread put it).
 template <typename T, bool RES>
 __global__ __launch_bounds__(1024) void rmsnorm_fwd_long_kernel(const T* x, const T* res, const T* __restrict__ w, T eps, T* h, T* y,
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_fwd_long_kernel(const T* x, cons
 template <typename T, int V, int NT, int E>
 int launch_fwd(fx_ctx* c, const T* x, const T* res, const T* w, T eps, T* h, T* y, T* rstd, i64 rows, i64 D) {
     constexpr int BT = block_of(NT);
-    constexpr i64 MOST = (1ll << 22) * (BT / NT);  // rows of one launch, which has fewer than 2^32 threads
+    constexpr i64 MOST = 0xffffffffll / BT * (BT / NT);  // rows of one launch, which has fewer than 2^32 threads
     const dim3 blk(BT);
     for (i64 r = 0; r < rows; r += MOST) {
         const i64 n = std::min(rows - r, MOST), at = r * D;
@@ -133,10 +135,14 @@ int rmsnorm_fwd(fx_ctx* c, const T* x, const T* res, const T* w, double eps, T* 
     constexpr int V = 16 / (int)sizeof(T);
     const T e = (T)eps;
     if (D > 1024 * 16) {
-        const dim3 grid((unsigned)rows), blk(1024);
-        if (res) FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, e, h, y, rstd, D), rmsnorm_fwd_long_kernel<T, true>);
-        else FX_LAUNCH(grid, blk, 0, c->stream, (x, res, w, e, h, y, rstd, D), rmsnorm_fwd_long_kernel<T, false>);
-        FX_LAUNCH_CHECK();
+        for (i64 r = 0; r < rows; r += MOST_LONG) {
+            const dim3 grid((unsigned)std::min(rows - r, MOST_LONG)), blk(1024);
+            const i64 at = r * D;
+            T* const rs = rstd ? rstd + r : nullptr;
+            if (res) FX_LAUNCH(grid, blk, 0, c->stream, (x + at, res + at, w, e, h + at, y + at, rs, D), rmsnorm_fwd_long_kernel<T, true>);
+            else FX_LAUNCH(grid, blk, 0, c->stream, (x + at, nullptr, w, e, nullptr, y + at, rs, D), rmsnorm_fwd_long_kernel<T, false>);
+            FX_LAUNCH_CHECK();
+        }
         return FX_OK;
     }
     return dispatch_fwd<T, V>(c, x, res, w, e, h, y, rstd, rows, D);
@@ -292,8 +298,12 @@ int rmsnorm_bwd(fx_ctx* c, const T* dy, const T* dh, const T* h, const T* w, con
                 if (int rc = column_sum<T>(c, part, dw, (int)slices, D)) return rc;
             }
         }
-        FX_LAUNCH(dim3((unsigned)rows), dim3(1024), 0, c->stream, (dy, dh, h, w, rstd, dx, D), rmsnorm_bwd_long_kernel<T>);
-        FX_LAUNCH_CHECK();
+        for (i64 r = 0; r < rows; r += MOST_LONG) {
+            const i64 at = r * D;
+            FX_LAUNCH(dim3((unsigned)std::min(rows - r, MOST_LONG)), dim3(1024), 0, c->stream,
+                      (dy + at, dh ? dh + at : nullptr, h + at, w, rstd + r, dx + at, D), rmsnorm_bwd_long_kernel<T>);
+            FX_LAUNCH_CHECK();
+        }
         return FX_OK;
     }
     return dispatch_bwd<T, V>(c, dy, dh, h, w, rstd, dx, dw, rows, D);
