@@ -623,7 +623,7 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const T* __restrict_
 template <typename T, class Cfg, class AL, class BL, class EP>
 int launch(fx_ctx* c, const AL& al, const BL& bl, const EP& ep, i64 M, i64 N, i64 K, int splits, int kps) {
     const i64 gx = fx::ceil_div(N, Cfg::BN), gy = fx::ceil_div(M, Cfg::BM);
-    FX_REQUIRE(gx <= 0x7fffffff && gy <= 65535 && splits >= 1 && splits <= 65535, "implicit GEMM grid out of range");
+    FX_REQUIRE(gx * Cfg::NT < (1ll << 32) && gy <= 65535 && splits >= 1 && splits <= 65535, "implicit GEMM grid out of range");
     FX_REQUIRE(K >= 1, "implicit GEMM needs K >= 1");
     FX_LAUNCH(dim3((unsigned)gx, (unsigned)gy, (unsigned)splits), dim3(Cfg::NT), 0, c->stream, (
         al, bl, ep, (int)K, kps), igemm_kernel<T, Cfg, AL, BL, EP>);
@@ -752,13 +752,13 @@ int launch_splitk_reduce_pair(fx_ctx* c, const T* part, i64 stride, int splits, 
 
 template <typename T>
 __global__ __launch_bounds__(256) void zero_kernel(T* __restrict__ out, i64 n) {
-    const i64 i = (i64)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) out[i] = T(0);
+    for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < n; i += (i64)gridDim.x * 256) out[i] = T(0);
 }
 template <typename T>
 int launch_zero(fx_ctx* c, T* out, i64 n) {
     if (n == 0) return FX_OK;
-    FX_LAUNCH(dim3((unsigned)fx::ceil_div(n, 256)), dim3(256), 0, c->stream, (out, n), zero_kernel<T>);
+    const i64 blocks = std::min<i64>(fx::ceil_div(n, (i64)256), 1 << 23);  // a launch has fewer than 2^32 threads
+    FX_LAUNCH(dim3((unsigned)blocks), dim3(256), 0, c->stream, (out, n), zero_kernel<T>);
     FX_LAUNCH_CHECK();
     return FX_OK;
 }

@@ -41,7 +41,8 @@ def run(exe, cases):
 # elements -.
 TAKEN = {
     "GEMM": [("linear", t, m, n, k) for t in ("f32", "f64") for m, n, k in ((1, (1 << 26) - 4, 2), (1, (1 << 26) - 3, 2), (1, (1 << 26) - 1, 1), (1, 1 << 26, 2),
-                                                                          (4, (1 << 26) - 1, 512), (2, 70000000, 513), (4000000, 1, 2), (1, 1, 1 << 20))],
+                                                                          (4, (1 << 26) - 1, 512), (2, 70000000, 513), (4000000, 1, 2), (1, 1, 1 << 20),
+                                                                          (70000, 70000, 0), (1, 1 << 30, 0))],
     "NORM": [(c, t, r, d, 0) for t in ("f32", "f64") for c in ("norm", "norm_res", "norm_bwd")
              for r, d in ((B31, 1), (1 << 26, 257), ((1 << 26) + 1, 256), (1 << 24, 2049), (1 << 22, 4097), ((1 << 22) - 1, 4097), ((1 << 23) + 1, 4098),
                           (1 << 22, 16384), (1 << 22, 16385), ((1 << 22) + 7, 16390), (3, B31), (1, B31))],
@@ -62,7 +63,8 @@ def test_sizes_that_one_launch_cannot_hold(binaries, part):
 
 def test_sizes_that_are_refused(binaries):
     """With a message, before anything is launched that could not run."""
-    cases = {"EMBED": [("embed_bwd", "f32", 100, 1 << 30, 1), ("embed_bwd", "f32", 3, 2, 1 << 25), ("embed_bwd", "f64", 3, 2, 1 << 24), ("embed", "f32", 1 << 31, 2, 2)],
+    cases = {"GEMM": [("linear", "f32", 70000000, 1, 2), ("linear", "f32", 5, B31, 1)],
+             "EMBED": [("embed_bwd", "f32", 100, 1 << 30, 1), ("embed_bwd", "f32", 3, 2, 1 << 25), ("embed_bwd", "f64", 3, 2, 1 << 24), ("embed", "f32", 1 << 31, 2, 2)],
              "SCAN": [("scan", "f32", 1, 1 << 30, 1), ("scan_bwd", "f64", 1, 1 << 28, 1), ("scan", "f32", 4, 1, 1 << 30)]}
     for part, list_ in cases.items():
         for case, said in zip(list_, run(binaries[part], list_)):
