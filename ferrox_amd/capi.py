@@ -666,10 +666,13 @@ class Context:
 
     # ---- a language model's training step (`out`: the caller's own output arrays, None: from the pool)
     def upload_ids(self, ids):
-        """Token ids on the device (int64) for embedding_fwd / embedding_bwd; any shape, read in order."""
+        """Token ids (whole numbers) on the device as int64 for embedding_fwd / embedding_bwd; any shape, read in order."""
+        ids = np.asarray(ids)
+        if ids.size and ids.dtype.kind not in "iu":
+            raise FerroxHipError(1, f"upload_ids: ids are {ids.dtype}, not whole numbers")
         ids = np.ascontiguousarray(ids, dtype=np.int64)
         d = _RawI64(self, max(1, ids.size))
-        d.shape = ids.shape
+        d.shape, d.n = ids.shape, ids.size
         if ids.size:
             check(lib.fx_h2d(self.h, d.ptr, ids.ctypes.data_as(_vp), ids.nbytes))
         return d
