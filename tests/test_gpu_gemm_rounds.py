@@ -22,3 +22,16 @@ def test_products_of_several_rounds(ctx, m, k, n):
     for ta, tb in ((False, True), (False, False), (True, False), (True, True)):
         got = ctx.gemm(ctx.upload(A.T if ta else A), ctx.upload(B.T if tb else B), ta, tb).numpy()
         assert (np.abs(got - y) <= bound).all(), (ta, tb)
+
+
+@pytest.mark.parametrize("m,k,n", [(4092, 192, 1020), (4090, 260, 1021), (4095, 132, 1023), (8192, 128, 900)])
+def test_epilogue_in_128_x_64_tiles(ctx, m, k, n):
+    rng = np.random.default_rng(m + k)
+    A, B = rng.standard_normal((m, k)).astype(np.float32), (rng.standard_normal((k, n)) / np.sqrt(k)).astype(np.float32)
+    bias, res = rng.standard_normal(n).astype(np.float32), rng.standard_normal((m, n)).astype(np.float32)
+    for (ta, tb), act in zip(((False, True), (False, False), (True, False), (True, True)), ("gelu", "none", "silu", "relu")):
+        pre = ctx.empty((m, n))
+        got = ctx.gemm_bias_act_residual(ctx.upload(A.T if ta else A), ctx.upload(B.T if tb else B), ta, tb, bias=ctx.upload(bias), act=act,
+                                         residual=ctx.upload(res), pre=pre).numpy()
+        y, p, by, bp = ref.linear_fwd(A, B, bias, act, res)
+        assert (np.abs(got - y) <= by).all() and (np.abs(pre.numpy() - p) <= bp).all(), (ta, tb, act)
