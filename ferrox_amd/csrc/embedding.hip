@@ -90,7 +90,7 @@ __device__ __forceinline__ void rank_items(const uint32_t (&key)[K], int shift, 
 }
 
 // counts [wave][bin] -> where the items of (bin, wave) start among the block's items: an exclusive scan in (bin, wave) order.
-// totals (optional): the block's items per bin.  wsum: 4 values.  Barriers on both sides.
+// wsum: 4 values.  Barriers on both sides.
 __device__ __forceinline__ void scan_counts(uint32_t* counts, uint32_t* wsum) {
     __syncthreads();
     const int t = threadIdx.x, lane = t & 63;

@@ -529,7 +529,7 @@ inline Plan make_plan(int num_cus, bool ta, bool tb, i64 M, i64 N, i64 K, i64 ld
     if (K < 2 * KC || (K % KC != 0 && !(K % 4 == 0 && !ta && tb)) || lda % 4 != 0 || ldb % 4 != 0 || M < 64 || N < 64) return pl;
     if ((ta && M % 4 != 0) || (!tb && N % 4 != 0)) return pl;
     // tile shape: the one with the least (rounds of co-resident blocks) x (work of a block); a nearly empty last round
-    // costs as much as a full one (3072 x 3072: 576 tiles of 128 x 128 take two rounds, 1152 of 128 x 64 take 2.25).  The
+    // costs as much as a full one (3000 x 3000: 576 tiles of 128 x 128 take two rounds, 1128 of 128 x 64 take 2.2).  The
     // work of a block is its MFMA count weighted by what the tile reads per MFMA (narrower tiles re-read more).
     const i64 slots = 2 * (i64)std::max(1, num_cus);
     static const int shapes[4][3] = {{4, 4, 8}, {4, 2, 9}, {2, 2, 10}, {2, 1, 11}};  // WM, TN, cost per 32 x 32 block

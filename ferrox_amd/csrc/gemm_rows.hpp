@@ -86,7 +86,8 @@ __global__ __launch_bounds__(NT) void rows_kernel(const T* __restrict__ A, const
 
 // One row always; up to four where K is long enough to hide the M x RN sums' trees.  Measured at K = N = 4096 against the small-product
 // kernel (us): f32 1 row 12.0 (67 MB at 5.6 TB/s) / 26.1, 2 rows 13.0 / 26.2, 4 rows 15.4 / 26.3, 8 rows 20.1 / 26.8; f64 23.8 / 43.6, 26.5 /
-// 44.0, 29.9 / 45.2, 55.9 / 46.8.  4 rows at K = 128, N = 4096: 7.9 / 5.4, and 8 rows at K = 512, N = 256: 8.9 / 5.6.
+// 44.0, 29.9 / 45.2, 55.9 / 46.8.  4 rows at K = 128, N = 4096: 7.9 / 5.4, and 8 rows at K = 512, N = 256: 8.9 / 5.6.  Eight rows gain in
+// f32 with long K and N alone; they would need a rule of their own and are left to the other kernels.
 // A launch has fewer than 2^32 threads, 256 for four rows of B.
 inline bool eligible(bool ta, bool tb, i64 M, i64 N, i64 K) {
     return !ta && tb && K >= 1 && K < (1ll << 30) && N <= (1ll << 26) - 4 && (M == 1 || (M <= 4 && K >= 512));

@@ -13,8 +13,8 @@
 // also publishes the state it ended in, so that no block collects more than GROUP maps).
 //   - Which piece of its 64 chains a block runs is its ticket from a counter that these chains have to themselves (one counter for all
 //     served 80 blocks per microsecond and bounded the launch), so every piece it waits for has been taken by a block that is running
-//     already and publishes after a bounded amount of work of its own: every wait ends.  (A wait that lasts for millions of polls all
-//     the same gives up and yields NaN instead of hanging.)
+//     already and publishes after a bounded amount of work of its own: every wait ends.  (A wait that lasted for millions of polls all
+//     the same would give up and yield NaN instead of hanging; by the order of the tickets none can.)
 //   - A published value is whole in one 64-bit word (f32: A and H; f64: one word each), written and read by relaxed device-scope
 //     atomics; no other memory is handed over, so no fence is needed.  Words start as all ones, a pattern that no published value has
 //     (NaNs are replaced by the standard one first); a small kernel sets them and the counters before every launch.

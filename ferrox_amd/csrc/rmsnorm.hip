@@ -3,9 +3,11 @@
 //   backward:  dx_j = dh_j + rstd (w_j dy_j) - h_j rstd^3 (sum_k w_k dy_k h_k) / D;  dw_j = sum over rows of dy_j (h_j rstd)
 // Both are bound by memory: 2 reads and 2 writes of [rows, D] forward, 3 reads and 1 write backward.  A row stays in registers
 // between its one read and its one write: up to 16 elements per thread, one wave per row up to 1024 elements, a block of 256 up to
-// 4096 and of 1024 up to 16384; longer rows are read twice.  All accesses are 16-byte vectors that start at any element (a row of an
-// odd length moves the next one off the 16-byte grid); only the last, incomplete vector of a row goes element by element.  Sums are held in the
-// tensors' own type (f32 or f64): a thread adds at most 16 terms before the tree of its block.
+// 4096 and of 1024 up to 16384.  All accesses to such rows are 16-byte vectors that start at any element (a row of an odd length moves the
+// next one off the 16-byte grid); only the last, incomplete vector of a row goes element by element.  Sums are held in the tensors' own
+// type (f32 or f64): of such a row a thread adds at most 16 terms before the tree of its block.  Longer rows are read twice, element by
+// element, and a thread adds one term in 1024 of the row, one after the other.  Rows of a few elements leave most of their wave idle and
+// are bound by its latency.
 // The weight gradient is added up in registers over the rows that a block takes (thread t owns the same columns in every row), one
 // partial row per block, and the partial rows are added by a second launch in a fixed order: no atomics.
 #include <mutex>

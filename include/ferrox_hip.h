@@ -391,8 +391,9 @@ enum fx_scalar_op { FX_ADD_SCALAR = 0, FX_SUB_SCALAR = 1, FX_MUL_SCALAR = 2, FX_
     int fx_sgd_step_multi_##S(fx_ctx* ctx, int count, T* const* p, const T* const* g, const int64_t* n, T lr);         \
     int fx_sgd_momentum_step_multi_##S(fx_ctx* ctx, int count, T* const* p, const T* const* g, T* const* buf,          \
                                        const int64_t* n, T lr, T momentum, T weight_decay, int nesterov);               \
-    /* ---- a language model's training step ----  The reference trains image classifiers and has none of these; they sit\
-       beside its layers, losses and optimizers in the same form.  All tensors are dense, token ids are int64 on the device.\
+    /* ---- a language model's training step ----  The reference trains image classifiers; of these it has the clipping\
+       alone (SGD::clip_grad_norm, src/nn/optim/sgd.rs:56-101).  They sit beside its layers, losses and optimizers in the\
+       same form.  All tensors are dense, token ids are int64 on the device, sums are held in T where nothing else is said.\
                                                                                                                        \
        Embedding lookup and its weight gradient.  fwd: out[n, :] = scale * W[ids[n], :]; an id outside 0 .. vocab - 1  \
        (padding) gives a row of zeros.  bwd: dW[v, :] = scale * the sum of g[n, :] over the n with ids[n] = v; every row of\
@@ -438,7 +439,8 @@ enum fx_scalar_op { FX_ADD_SCALAR = 0, FX_SUB_SCALAR = 1, FX_MUL_SCALAR = 2, FX_
        written then where nothing is scaled), and shares memory with no other tensor of the call.  Squares are added in\
        double for both types, in a fixed order; finite gradients of any magnitude are clipped by their norm, also where\
        norm[0] lies beyond the type and reads infinity.  Where an element is infinite or NaN, so is norm[0], and nothing\
-       is scaled.  No host synchronisation: the calls may be recorded (fx_graph_*). */                                 \
+       is scaled (the reference multiplies by max_norm/infinity = 0 there).  No host synchronisation: the calls may be \
+       recorded (fx_graph_*). */                                                                                       \
     int fx_grad_norm_multi_##S(fx_ctx* ctx, int count, const T* const* g, const int64_t* n, T* norm);                  \
     int fx_clip_grad_norm_multi_##S(fx_ctx* ctx, int count, const T* const* g, T* const* out, const int64_t* n,        \
                                     double max_norm, T* norm);
