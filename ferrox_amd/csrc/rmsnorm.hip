@@ -1,6 +1,6 @@
 // Root-mean-square norm over the rows of [rows, D] with the residual's addition in front of it, and its backward pass.
 //   forward:   h = x + res;  rstd = (sum_j h_j^2 / D + eps)^(-1/2);  y_j = (h_j rstd) w_j
-//   backward:  dx_j = dh_j + rstd (w_j dy_j) - h_j rstd^3 (sum_k w_k dy_k h_k) / D;  dw_j = sum over rows of dy_j (h_j rstd)
+//   backward:  with n_j = h_j rstd, dx_j = dh_j + rstd (w_j dy_j - n_j (sum_k w_k dy_k n_k) / D);  dw_j = sum over rows of dy_j n_j
 // Both are bound by memory: 2 reads and 2 writes of [rows, D] forward, 3 reads and 1 write backward.  A row stays in registers
 // between its one read and its one write: up to 16 elements per thread, one wave per row up to 1024 elements, a block of 256 up to
 // 4096 and of 1024 up to 16384.  All accesses to such rows are 16-byte vectors that start at any element (a row of an odd length moves the
@@ -8,6 +8,8 @@
 // type (f32 or f64): of such a row a thread adds at most 16 terms before the tree of its block.  Longer rows are read twice, element by
 // element, and a thread adds one term in 1024 of the row, one after the other.  Rows of a few elements leave most of their wave idle and
 // are bound by its latency.
+// Rows whose squares leave the type's range (their mean overflows, or is so small that squares may have vanished) are summed once more
+// with their elements times a power of two; the branch is uniform over a row.
 // The weight gradient is added up in registers over the rows that a block takes (thread t owns the same columns in every row), one
 // partial row per block, and the partial rows are added by a second launch in a fixed order: no atomics.
 #include <mutex>
@@ -20,6 +22,14 @@ using namespace vio;
 template <typename T> __device__ __forceinline__ T inv_sqrt(T v);
 template <> __device__ __forceinline__ float inv_sqrt<float>(float v) { return 1.f / sqrtf(v); }
 template <> __device__ __forceinline__ double inv_sqrt<double>(double v) { return 1. / sqrt(v); }
+
+// Means of squares between these are taken as they are; below, the row counts UP-fold (an eps that matters there does not overflow by
+// it), above and for NaN it counts DOWN-fold.
+template <typename T> struct Range;
+template <> struct Range<float> { static constexpr float LO = 0x1p-100f, HI = 0x1.fffffep127f, UP = 0x1p100f, DOWN = 0x1p-80f; };
+template <> struct Range<double> { static constexpr double LO = 0x1p-900, HI = 0x1.fffffffffffffp1023, UP = 0x1p600, DOWN = 0x1p-600; };
+template <typename T> __device__ __forceinline__ bool in_range(T mean) { return mean >= Range<T>::LO && mean <= Range<T>::HI; }
+template <typename T> __device__ __forceinline__ T rescue(T mean) { return mean < Range<T>::LO ? Range<T>::UP : Range<T>::DOWN; }
 
 constexpr int block_of(int nt) { return nt < 256 ? 256 : nt; }
 
@@ -53,8 +63,25 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_fwd_kernel(const T* x, c
 #pragma unroll
         for (int u = 0; u < V; ++u) s = s + v[k][u] * v[k][u];
     s = block_sum<NT>(s, sm);
-    const T r = inv_sqrt<T>(s / T(D) + eps);
-    if (t == 0 && rstd) rstd[row] = r;
+    const T mean = s / T(D) + eps;
+    T r, f = T(1);
+    if (in_range(mean)) {
+        r = inv_sqrt<T>(mean);
+    } else {
+        f = rescue(mean);
+        s = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                v[k][u] = v[k][u] * f;
+                s = s + v[k][u] * v[k][u];
+            }
+        if (NT > 64) __syncthreads();  // the sums before have been read
+        s = block_sum<NT>(s, sm);
+        r = inv_sqrt<T>(s / T(D) + eps * f * f);
+    }
+    if (t == 0 && rstd) rstd[row] = r * f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         T g[V];
@@ -83,10 +110,24 @@ __global__ __launch_bounds__(1024) void rmsnorm_fwd_long_kernel(const T* x, cons
         s = s + v * v;
     }
     s = block_sum<1024>(s, sm);
-    const T r = inv_sqrt<T>(s / T(D) + eps);
-    if (threadIdx.x == 0 && rstd) rstd[blockIdx.x] = r;
     const T* src = RES ? h : x;
-    for (i64 j = threadIdx.x; j < D; j += 1024) y[base + j] = (src[base + j] * r) * w[j];
+    const T mean = s / T(D) + eps;
+    T r, f = T(1);
+    if (in_range(mean)) {
+        r = inv_sqrt<T>(mean);
+    } else {
+        f = rescue(mean);
+        s = T(0);
+        for (i64 j = threadIdx.x; j < D; j += 1024) {
+            const T v = src[base + j] * f;
+            s = s + v * v;
+        }
+        __syncthreads();  // the sums before have been read
+        s = block_sum<1024>(s, sm);
+        r = inv_sqrt<T>(s / T(D) + eps * f * f);
+    }
+    if (threadIdx.x == 0 && rstd) rstd[blockIdx.x] = r * f;
+    for (i64 j = threadIdx.x; j < D; j += 1024) y[base + j] = ((src[base + j] * f) * r) * w[j];
 }
 
 template <typename T, int V, int NT, int E>
@@ -180,13 +221,14 @@ __global__ __launch_bounds__(block_of(NT)) void rmsnorm_bwd_kernel(const T* dy, 
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int u = 0; u < V; ++u) {
-                dw[k][u] = dw[k][u] + g[k][u] * (hv[k][u] * r);
+                hv[k][u] = hv[k][u] * r;
+                dw[k][u] = dw[k][u] + g[k][u] * hv[k][u];
                 g[k][u] = g[k][u] * wv[k][u];
                 s = s + g[k][u] * hv[k][u];
             }
         if (GR == 1) __syncthreads();  // the sums of the row before have been read
         s = block_sum<NT>(s, sm);
-        const T q = (s / T(D)) * (r * r);
+        const T q = s / T(D);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             T d[V];
@@ -226,11 +268,11 @@ __global__ __launch_bounds__(1024) void rmsnorm_bwd_long_kernel(const T* dy, con
     const i64 base = (i64)blockIdx.x * D;
     const T r = rstd[blockIdx.x];
     T s = T(0);
-    for (i64 j = threadIdx.x; j < D; j += 1024) s = s + (dy[base + j] * w[j]) * h[base + j];
+    for (i64 j = threadIdx.x; j < D; j += 1024) s = s + (dy[base + j] * w[j]) * (h[base + j] * r);
     s = block_sum<1024>(s, sm);
-    const T q = (s / T(D)) * (r * r);
+    const T q = s / T(D);
     for (i64 j = threadIdx.x; j < D; j += 1024) {
-        const T a = r * (dy[base + j] * w[j] - h[base + j] * q);
+        const T a = r * (dy[base + j] * w[j] - (h[base + j] * r) * q);
         dx[base + j] = dh ? a + dh[base + j] : a;
     }
 }
