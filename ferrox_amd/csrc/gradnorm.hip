@@ -79,12 +79,25 @@ struct Squares {
     }
 };
 
+// block_sum of v, and whether any thread is marked: one barrier for both.
+__device__ __forceinline__ double block_sum_marked(double v, bool& marked, double* sm, int* marks) {
+    const bool wave = __any(marked);
+    if ((threadIdx.x & 63) == 0) marks[threadIdx.x >> 6] = wave;
+    v = block_sum<NT>(v, sm);
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) all |= marks[w];
+    marked = all != 0;
+    return v;
+}
+
 // part: 3 planes of `plane` partial sums (f32: the first one only)
 template <typename T>
 __global__ __launch_bounds__(NT) void sum_squares_kernel(const Tensors<T> tt, double* __restrict__ part, i64 plane) {
     constexpr int V = 16 / (int)sizeof(T), PER = CHUNK / NT / V;
     constexpr bool WIDE = sizeof(T) == 8;
     __shared__ double sm[3][NT / 64 + 1];
+    __shared__ int marks[NT / 64];
     __shared__ Table<T> tab;
     const Starts starts = stage_table(tt, tab);
     Squares s;
@@ -119,9 +132,10 @@ __global__ __launch_bounds__(NT) void sum_squares_kernel(const Tensors<T> tt, do
             }
         }
     }
-    double mid = block_sum<NT>(s.mid, sm[0]);
+    bool outer = WIDE && !(s.large == 0. && s.small == 0.);
+    double mid = WIDE ? block_sum_marked(s.mid, outer, sm[0], marks) : block_sum<NT>(s.mid, sm[0]);
     if constexpr (WIDE) {
-        if (__syncthreads_or(!(s.large == 0. && s.small == 0.))) {
+        if (outer) {
             mid = -mid;  // minus zero as well
             const double large = block_sum<NT>(s.large, sm[1]), small = block_sum<NT>(s.small, sm[2]);
             if (threadIdx.x == 0) {
@@ -140,16 +154,17 @@ struct Norm {  // root * 2^e
 };
 // The norm from all partials, the same bits in every block.
 template <bool WIDE> __device__ __forceinline__ Norm norm_of(const double* __restrict__ part, i64 plane, int parts, double (*sm)[NT / 64 + 1]) {
+    __shared__ int marks[NT / 64];
     double s = 0.;
-    int marked = 0;
+    bool marked = false;
     for (int j = threadIdx.x; j < parts; j += NT) {
         const double p = part[j];
         marked |= __double2hiint(p) < 0;
         s = s + fabs(p);
     }
-    s = block_sum<NT>(s, sm[0]);
+    s = WIDE ? block_sum_marked(s, marked, sm[0], marks) : block_sum<NT>(s, sm[0]);
     if constexpr (WIDE) {
-        if (__syncthreads_or(marked)) {
+        if (marked) {
             double large = 0., small = 0.;
             for (int j = threadIdx.x; j < parts; j += NT) {
                 if (__double2hiint(part[j]) >= 0) continue;

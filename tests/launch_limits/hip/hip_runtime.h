@@ -9,7 +9,6 @@ inline unsigned long long __ballot(int) { return 0; }
 inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 inline int __ffsll(unsigned long long v) { return __builtin_ffsll((long long)v); }
 inline int __any(int v) { return v; }
-inline int __syncthreads_or(int v) { return v; }
 inline unsigned atomicAdd(unsigned* p, unsigned v) { const unsigned o = *p; *p += v; return o; }
 inline float __uint_as_float(uint32_t v) { float f; memcpy(&f, &v, 4); return f; }
 inline uint32_t __float_as_uint(float f) { uint32_t v; memcpy(&v, &f, 4); return v; }
