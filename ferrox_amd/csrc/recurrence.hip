@@ -19,8 +19,8 @@
 //     atomics; no other memory is handed over, so no fence is needed.  Words start as all ones, a pattern that no published value has
 //     (NaNs are replaced by the standard one first); a small kernel sets them and the counters before every launch.
 //   - Maps are folded in the order of the pieces, whenever they arrive: the result does not depend on timing.
-// Measured (MI355X): 2 x 8192 x 1024 f32 forward 49 us with the clearing, 201 MB at 4.1 TB/s (two launches, the first composing the maps of
-// all pieces and reading the inputs once more: 75 us); 16 x 511 x 1000 f64 backward 88 us, 393 MB at 4.5 TB/s (one block per 64 chains
+// Measured (MI355X): 2 x 8192 x 1024 f32 forward 50 us with the clearing, 201 MB at 4.0 TB/s (two launches, the first composing the maps of
+// all pieces and reading the inputs once more: 75 us); 16 x 511 x 1000 f64 backward 90 us, 393 MB at 4.4 TB/s (one block per 64 chains
 // that walks the axis: 106 us).
 #include <mutex>
 #include <type_traits>
